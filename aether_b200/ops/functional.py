@@ -779,3 +779,207 @@ def head_rmsnorm_(x, h0, nh, D, w, eps=1e-6):
     v = v * torch.rsqrt(v.pow(2).mean(-1, keepdim=True) + eps) * w.float()
     x[:, h0 * D : (h0 + nh) * D] = v.reshape(x.shape[0], -1).to(x.dtype)
     return x
+
+
+# ------------------------------------------------------------------ 8-bit paged KV cache
+KV8_BLOCK = ref.KV8_BLOCK
+KV8_WORKSPACE = 16 << 20
+
+
+def kv8_workspace(device):
+    """Scratch of ``kv8_decode_attention`` (any shapes): zeroed once; every call
+    leaves its counters zero again. One call at a time may use it."""
+    return torch.zeros(KV8_WORKSPACE, dtype=torch.uint8, device=device)
+
+
+def _kv8_rows(x, name):
+    if x.dim() != 2 or x.dtype != BF16:
+        raise ValueError(f"{name}: bf16 [rows, width]")
+    return x
+
+
+def rope_kv8_append(qkv, pos, slot, cos_t, sin_t, kc, ks, vc, vs, page_table, Hq, row_start=None, out=None):
+    """Rotates the q and k heads of qkv [T, >= (Hq + 2 Hkv) D] and appends k and v
+    to an 8-bit paged cache: codes uint8 [pages, Hkv, page, D] (code + 128) and
+    scales fp32 [pages, Hkv, page / 16]; 16 consecutive positions of a sequence
+    share one scale for each head.
+
+    Sequence b takes rows row_start[b] .. row_start[b + 1] (None: row b alone) at
+    positions pos[b] .. of page-table row slot[b] (negative: skipped); a sequence
+    appears once. What the block of pos[b] held from pos[b] on is forgotten; its
+    older positions are rounded again when the scale grows. The rotated q and k
+    go to out [T, >= (Hq + Hkv) D], or back into qkv. A non-finite k or v makes
+    its block read as NaN."""
+    if out is None:
+        out = qkv
+    if _cuda(qkv):
+        C().rope_kv8_append(qkv, pos, slot, row_start, cos_t, sin_t, kc, ks, vc, vs, page_table, Hq, out)
+        return out
+    _kv8_rows(qkv, "rope_kv8_append: qkv")
+    Hkv, D = kc.shape[1], kc.shape[3]
+    if row_start is None and qkv.shape[0] != pos.shape[0]:
+        raise ValueError("rope_kv8_append: without row_start, one row of qkv for each sequence")
+    for b in range(pos.shape[0]):
+        r0, r1 = (b, b + 1) if row_start is None else (int(row_start[b]), int(row_start[b + 1]))
+        if int(slot[b]) < 0 or r1 <= r0:
+            continue
+        p0 = int(pos[b])
+        x = qkv[r0:r1].float()
+        y = ref.rope(x, torch.arange(p0, p0 + r1 - r0), cos_t, sin_t, Hq + Hkv, D)
+        heads = y[:, : (Hq + 2 * Hkv) * D].view(r1 - r0, Hq + 2 * Hkv, D)
+        pages = page_table[int(slot[b])]
+        ref.kv8_store(heads[:, Hq : Hq + Hkv], p0, kc, ks, pages)
+        ref.kv8_store(heads[:, Hq + Hkv :], p0, vc, vs, pages)
+        out[r0:r1, : (Hq + Hkv) * D] = y[:, : (Hq + Hkv) * D].to(out.dtype)
+    return out
+
+
+def gather_kv8(codes, scale, page_table, slot, first, n, out=None):
+    """bf16 [B, n, Hkv, D]: positions first .. first + n (``first`` an int for all
+    or int32 [B]) of page-table rows slot [B] of an 8-bit pool. Positions that
+    the table does not reach read as zero."""
+    if out is None:
+        out = torch.empty(slot.shape[0], n, codes.shape[1], codes.shape[3], dtype=BF16, device=codes.device)
+    if _cuda(codes):
+        if isinstance(first, torch.Tensor):
+            C().gather_kv8(codes, scale, page_table, slot, first, 0, out)
+        else:
+            C().gather_kv8(codes, scale, page_table, slot, None, first, out)
+        return out
+    for b in range(slot.shape[0]):
+        f = int(first[b]) if isinstance(first, torch.Tensor) else int(first)
+        v = ref.kv8_values(codes, scale, page_table[int(slot[b])], f + n)[f:]
+        out[b].zero_()
+        out[b, : v.shape[0]] = v.to(BF16)
+    return out
+
+
+def kv8_decode_attention(q, kc, ks, vc, vs, page_table, slot, seqlen, Hq, scale, out=None, workspace=None, window=0,
+                         softcap=0.0):
+    """Attention of one new token for each sequence over an 8-bit paged cache
+    (pools as in ``rope_kv8_append``): q [B, >= Hq D], seqlen int32 [B] keys
+    (0, or slot < 0: the output row is zero) -> out bf16 [B, Hq D]. ``window``
+    > 0: the last ``window`` keys; ``softcap`` > 0: soft-capped logits.
+    ``workspace``: from ``kv8_workspace``, kept by the caller (a captured graph
+    must be given one); None allocates it."""
+    if out is None:
+        out = torch.empty(q.shape[0], Hq * kc.shape[3], dtype=BF16, device=q.device)
+    if _cuda(q):
+        C().kv8_decode_attention(q, kc, ks, vc, vs, page_table, slot, seqlen, out, Hq, scale, window, softcap)
+        return out
+    _kv8_rows(q, "kv8_decode_attention: q")
+    D = kc.shape[3]
+    for b in range(q.shape[0]):
+        L, s = int(seqlen[b]), int(slot[b])
+        if L <= 0 or s < 0:
+            out[b, : Hq * D] = 0
+            continue
+        k, v = (ref.kv8_values(c, z, page_table[s], L)[None] for c, z in ((kc, ks), (vc, vs)))
+        o, _ = ref.attention(q[b, : Hq * D].view(1, 1, Hq, D), k, v, scale, True, L - 1, window, softcap)
+        out[b, : Hq * D] = o.reshape(-1).to(out.dtype)
+    return out
+
+
+# ------------------------------------------------------------------ 4-bit weights with group scales
+W4_ROWS = 64  # rows that linear_w4 multiplies without expanding the weights
+
+
+class W4Weight:
+    """A projection [N, K] as packed 4-bit codes and fp16 scales, one for each
+    ``group`` (32, 64 or 128) columns of a row: value = (code - 8) * scale.
+    q int32 [ceil(N/16), ceil(K/128), 2, 32, 4] and s fp16
+    [ceil(N/16), ceil(K/128) * 128 / group, 8, 2], as ``pack_w4`` lays them out."""
+
+    __slots__ = ("q", "s", "N", "K", "group")
+
+    def __init__(self, q, s, N, K, group):
+        self.q, self.s, self.N, self.K, self.group = q, s, N, K, group
+
+    @property
+    def shape(self):
+        return torch.Size((self.N, self.K))
+
+    def bf16(self):
+        """The expanded bf16 [N, K] weight."""
+        return dequant_w4(self)
+
+    def bytes(self) -> int:
+        return self.q.numel() * 4 + self.s.numel() * 2
+
+    def to(self, device):
+        return W4Weight(self.q.to(device), self.s.to(device), self.N, self.K, self.group)
+
+
+def pack_w4(codes, scales):
+    """codes [N, K] of whole numbers 0..15 and scales [N, K / group] -> W4Weight."""
+    N, K = codes.shape
+    group = K // max(1, scales.shape[1])
+    if group not in (32, 64, 128) or K != group * scales.shape[1] or scales.shape[0] != N:
+        raise ValueError("pack_w4: scales [N, K / group] with a group of 32, 64 or 128")
+    return W4Weight(*ref.w4_pack(codes, scales), N, K, group)
+
+
+def quantize_w4(w, group=128):
+    """w [N, K] (K a multiple of group) -> W4Weight: scale = max |w| / 7 of each
+    group in fp16, code = round(w / scale) + 8."""
+    N, K = w.shape
+    if group not in (32, 64, 128) or K % group:
+        raise ValueError("quantize_w4: K is a multiple of the group (32, 64 or 128)")
+    g = w.float().view(N, K // group, group)
+    s = (g.abs().amax(-1) / 7).to(torch.float16)
+    f = s.float()[..., None]
+    c = torch.where(f > 0, g / f, torch.zeros_like(g)).round().clamp(-8, 7) + 8
+    return pack_w4(c.view(N, K).to(torch.int64), s)
+
+
+def dequant_w4(w, out=None):
+    """W4Weight -> bf16 [N, K] (each value rounded once)."""
+    if out is None:
+        out = torch.empty(w.N, w.K, dtype=BF16, device=w.q.device)
+    if _cuda(w.q):
+        C().dequant_w4(w.q, w.s, w.N, w.K, w.group, out)
+        return out
+    out.copy_(ref.w4_values(w.q, w.s, w.N, w.K, w.group).to(BF16))
+    return out
+
+
+def linear_w4(x, w, bias=None, residual=None, swiglu=False, out=None):
+    """y = x @ w^T (+ bias) (+ residual) for x bf16 [M, K] and a W4Weight [N, K];
+    swiglu: w = [gate; up] and y = silu(gate) * up, [M, N / 2]. Up to W4_ROWS
+    rows the 4-bit weights are multiplied as they are (exact codes, fp32 sums and
+    scales); more rows expand them to bf16 for the tensor-core GEMM."""
+    M = x.shape[0]
+    if out is None:
+        out = torch.empty(M, w.N // 2 if swiglu else w.N, dtype=BF16, device=x.device)
+    if _cuda(x):
+        if M <= W4_ROWS:
+            C().linear_w4(x, w.q, w.s, w.N, w.K, w.group, bias, residual, swiglu, out)
+        elif w.N % 8 == 0 and out.shape[1] % 8 == 0:
+            wb = dequant_w4(w)
+            if swiglu:
+                out.copy_(swiglu_residual(gemm(x, wb, bias=bias), residual))
+            else:
+                gemm(x, wb, bias=bias, residual=residual, out=out)
+        else:
+            for i in range(0, M, W4_ROWS):
+                r = slice(i, min(M, i + W4_ROWS))
+                C().linear_w4(x[r], w.q, w.s, w.N, w.K, w.group, bias, None if residual is None else residual[r],
+                              swiglu, out[r])
+        return out
+    if x.dim() != 2 or x.shape[1] != w.K:
+        raise ValueError("linear_w4: x is [M, K]")
+    y = x.float() @ ref.w4_values(w.q, w.s, w.N, w.K, w.group).t()
+    if bias is not None:
+        y = y + bias.float()
+    if swiglu:
+        y = ref.swiglu(y)
+    if residual is not None:
+        y = y + residual.float()
+    out.copy_(y.to(out.dtype))
+    return out
+
+
+def swiglu_residual(h, residual):
+    """silu(gate) * up of h = [gate, up] (+ residual)."""
+    a = swiglu(h)
+    return a if residual is None else a + residual

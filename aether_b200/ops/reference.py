@@ -130,3 +130,73 @@ def adamw(p, g, m, v, lr, beta1, beta2, eps, wd, step, gscale=1.0):
     vh = v / (1 - beta2**step)
     p.sub_(lr * (mh / (vh.sqrt() + eps) + wd * p))
     return p
+
+
+# ------------------------------------------------------------------ 8-bit paged KV cache
+KV8_BLOCK = 16
+
+
+def kv8_values(codes, scale, pages, length):
+    """fp32 [length, Hkv, D]: what the rows of ``pages`` (one sequence's physical
+    pages in order) of an 8-bit pool stand for."""
+    c = codes[pages.long()].float() - 128  # [n, Hkv, P, D]
+    v = c * scale[pages.long()].repeat_interleave(KV8_BLOCK, dim=2)[..., None]
+    return v.permute(0, 2, 1, 3).reshape(-1, c.shape[1], c.shape[3])[:length]
+
+
+def kv8_store(y, pos, codes, scale, pages):
+    """Quantises y [n, Hkv, D] fp32 into positions pos .. pos + n of the sequence
+    with the given physical pages: per block of 16 positions and head the scale
+    is max |new| / 127, or the block's older scale if that is larger and the
+    block holds older positions, whose codes are rounded again to it."""
+    n, P = y.shape[0], codes.shape[2]
+    t = pos
+    while t < pos + n:
+        base = t // KV8_BLOCK * KV8_BLOCK
+        end = min(pos + n, base + KV8_BLOCK)
+        page, row = int(pages[base // P]), base % P
+        part, old = y[t - pos : end - pos], t - base
+        s = part.abs().amax((0, 2)).clamp(min=2.0 ** -100) / 127
+        if old:
+            before = scale[page, :, row // KV8_BLOCK]
+            s = torch.maximum(before, s)
+            held = codes[page, :, row : row + old].float() - 128
+            held = (held * (before / s)[:, None, None]).nan_to_num(0.0).round()
+            codes[page, :, row : row + old] = (held + 128).to(torch.uint8)
+        new = (part * (1 / s)[None, :, None]).nan_to_num(0.0).round().clamp(-127, 127)
+        codes[page, :, row + old : row + old + end - t] = (new + 128).to(torch.uint8).transpose(0, 1)
+        scale[page, :, row // KV8_BLOCK] = s
+        t = end
+
+
+# ------------------------------------------------------------------ 4-bit weights with group scales
+W4_SHIFTS = (0, 16, 4, 20, 8, 24, 12, 28)
+
+
+def w4_pack(codes, scales):
+    """codes [N, K] (0..15; the value is (code - 8) * scale) and scales
+    [N, K / group] -> (q int32 [ceil(N/16), ceil(K/128), 2, 32, 4],
+    s fp16 [ceil(N/16), ceil(K/128) * 128 / group, 8, 2])."""
+    N, K = codes.shape
+    group = K // scales.shape[1]
+    nt, kt = -(-N // 16), -(-K // 128)
+    c = torch.full((nt * 16, kt * 128), 8, dtype=torch.int64, device=codes.device)
+    c[:N, :K] = codes
+    c = c.view(nt, 2, 8, kt, 4, 2, 4, 4).permute(0, 3, 1, 2, 6, 4, 5, 7).reshape(nt, kt, 2, 32, 4, 8)
+    q = torch.zeros(c.shape[:-1], dtype=torch.int64, device=codes.device)
+    for e, sh in enumerate(W4_SHIFTS):
+        q |= c[..., e] << sh
+    q = torch.where(q >= 1 << 31, q - (1 << 32), q).to(torch.int32)
+    s = torch.zeros(nt * 16, kt * 128 // group, dtype=torch.float16, device=codes.device)
+    s[:N, : K // group] = scales.to(torch.float16)
+    return q, s.view(nt, 2, 8, -1).permute(0, 3, 2, 1).contiguous()
+
+
+def w4_values(q, s, N, K, group):
+    """fp32 [N, K] of packed 4-bit weights."""
+    nt, kt = q.shape[:2]
+    sh = torch.tensor(W4_SHIFTS, device=q.device, dtype=torch.int32)
+    c = ((q[..., None] >> sh) & 15).view(nt, kt, 2, 8, 4, 4, 2, 4).permute(0, 2, 3, 1, 5, 6, 4, 7)
+    c = c.reshape(nt * 16, kt * 128 // group, group).float() - 8
+    f = s.float().permute(0, 3, 2, 1).reshape(nt * 16, -1, 1)
+    return (c * f).view(nt * 16, kt * 128)[:N, :K]

@@ -63,6 +63,19 @@ void attention_bwd(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, at:
 // attention_sm100.cu
 void attention_fwd_tc(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, std::optional<at::Tensor> lse,
                       double scale, bool causal, int64_t causal_offset, int64_t window, double softcap);
+// kv8.cu
+void rope_kv8_append(at::Tensor qkv, at::Tensor pos, at::Tensor slot, std::optional<at::Tensor> row_start,
+                     at::Tensor cos_t, at::Tensor sin_t, at::Tensor kc, at::Tensor ks, at::Tensor vc, at::Tensor vs,
+                     at::Tensor page_table, int64_t Hq, at::Tensor out);
+void gather_kv8(at::Tensor codes, at::Tensor scale, at::Tensor page_table, at::Tensor slot,
+                std::optional<at::Tensor> first, int64_t first0, at::Tensor out);
+void kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor vc, at::Tensor vs,
+                          at::Tensor page_table, at::Tensor slot, at::Tensor seqlen, at::Tensor out, int64_t Hq,
+                          double scale, int64_t window, double softcap);
+// w4.cu
+void linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group,
+               std::optional<at::Tensor> bias, std::optional<at::Tensor> residual, bool swiglu, at::Tensor y);
+void dequant_w4(at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group, at::Tensor out);
 // gemm_skinny.cu
 void skinny_gemm(at::Tensor x, at::Tensor w, at::Tensor acc, int64_t splits, int64_t acc_mc,
                  std::optional<at::Tensor> sig_peers, std::optional<at::Tensor> sig_epoch,
@@ -227,6 +240,11 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("head_rmsnorm", &aether::head_rmsnorm, "in-place per-head RMSNorm (Qwen3 q/k norm)");
   m.def("quantize_blocks", &aether::quantize_blocks, "bf16 -> GGUF Q8_0 (fmt 8) or Q4_0 (fmt 2) blocks");
   m.def("dequantize_blocks", &aether::dequantize_blocks, "GGUF Q8_0 / Q4_0 blocks -> bf16");
+  m.def("rope_kv8_append", &aether::rope_kv8_append, "RoPE, 8-bit quantisation and append to a paged cache");
+  m.def("gather_kv8", &aether::gather_kv8, "8-bit paged cache rows -> bf16");
+  m.def("kv8_decode_attention", &aether::kv8_decode_attention, "single-token attention over an 8-bit paged cache");
+  m.def("linear_w4", &aether::linear_w4, "a few rows times 4-bit weights with group scales");
+  m.def("dequant_w4", &aether::dequant_w4, "4-bit weights with group scales -> bf16");
   m.def("read_and_clear_status", &aether::read_and_clear_status,
         "Returns (and clears) the device status word set by kernels whose bounded waits expired");
 }

@@ -30,6 +30,7 @@ enum : int {
   kStatusTimeoutMma = 2,
   kStatusTimeoutEpilogue = 3,
   kStatusTimeoutPeer = 4,
+  kStatusKvRange = 5,  // a position, table row or page of a paged cache out of range
 };
 
 __device__ __forceinline__ uint32_t smem_u32(const void* p) {
