@@ -865,7 +865,9 @@ def kv8_decode_attention(q, kc, ks, vc, vs, page_table, slot, seqlen, Hq, scale,
     if out is None:
         out = torch.empty(q.shape[0], Hq * kc.shape[3], dtype=BF16, device=q.device)
     if _cuda(q):
-        C().kv8_decode_attention(q, kc, ks, vc, vs, page_table, slot, seqlen, out, Hq, scale, window, softcap)
+        if workspace is None:
+            workspace = kv8_workspace(q.device)
+        C().kv8_decode_attention(q, kc, ks, vc, vs, page_table, slot, seqlen, out, Hq, scale, workspace, window, softcap)
         return out
     _kv8_rows(q, "kv8_decode_attention: q")
     D = kc.shape[3]

@@ -71,7 +71,7 @@ void gather_kv8(at::Tensor codes, at::Tensor scale, at::Tensor page_table, at::T
                 std::optional<at::Tensor> first, int64_t first0, at::Tensor out);
 void kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor vc, at::Tensor vs,
                           at::Tensor page_table, at::Tensor slot, at::Tensor seqlen, at::Tensor out, int64_t Hq,
-                          double scale, int64_t window, double softcap);
+                          double scale, at::Tensor workspace, int64_t window, double softcap);
 // w4.cu
 void linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group,
                std::optional<at::Tensor> bias, std::optional<at::Tensor> residual, bool swiglu, at::Tensor y);

@@ -15,6 +15,7 @@
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
+#include <cuda_fp16.h>
 
 #include "common.cuh"
 #include "decode_common.cuh"
@@ -234,7 +235,40 @@ __global__ void __launch_bounds__(256) gather_kernel(Pool c, Map m, const int* _
 }
 
 // ------------------------------------------------------------------ attention
+// x_j = scale * s_k[j / 16] * sum_d q_d c_jd, p = softmax(x), o = sum_j p_j s_v[j / 16] c'_j
+//
+// Codes are exact in fp16, so both products run on the tensor cores with the
+// codes as they are and the scales outside: S^T = K q^T (16 keys x 8 query
+// heads of one KV head) and O^T = V^T w^T, as m16n8k16 steps whose operands come
+// straight from 16-byte global loads -- the order of the contraction is free, so
+// a thread's 16 consecutive codes are the k slots it owns, and no shared memory
+// is needed. q (8 significant bits) is exact in fp16 after a power-of-two scaling
+// of its row; the weight w_j = 2^(x_j + log2 s_v - M) carries the value scale, so
+// that fp16 (2^-11, range 2^-24 .. 2^14 around the running reference M) rounds
+// it relative to what it adds to the output. The denominator sums w_j / s_v in
+// fp32. M moves only when a weight would pass 2^4, so the accumulators are
+// rescaled a few times per sequence and not at every step.
+//
+// Bound by the cache's bytes. The 16-key blocks of all (sequence, KV head, eight
+// query heads) segments are laid end to end and cut into equal ranges, one for
+// each CTA (two of eight warps on an SM), so ragged batches fill the GPU; a
+// segment that one CTA holds whole is written at once, the parts of a cut one go
+// through the workspace and the last CTA to arrive joins them in order (a sum
+// that does not depend on who arrives when).
 constexpr float kLog2e = 1.4426950408889634f;
+constexpr int kWarps = 8;
+constexpr int kThreads = kWarps * 32;
+constexpr int kMaxCtas = 512;       // parts: two for each CTA
+constexpr int kMaxSegments = 65536; // counters
+constexpr int kMaxSeqs = 8192;
+constexpr int kMinSteps = 2;        // of kWarps blocks: shorter ranges cost more to join than they save
+constexpr float kWeightBits = 10.f; // weights are at most 2^(10 + 4) in fp16
+constexpr int kPartFloats = 8 * 128 + 16;
+constexpr int64_t kWorkspaceBytes = (int64_t)kMaxSegments * 4 + (int64_t)kMaxCtas * 2 * kPartFloats * 4;
+// dynamic shared memory: [8 warps][8 heads][128] sums (the parts' weights [8][kMaxCtas] in the join), their M and
+// l, block records, prefix of steps
+constexpr int kSmemSums = kWarps * 8 * 128 * 4;
+constexpr int kSmemFixed = kSmemSums + 2 * kWarps * 8 * 4 + kWarps * 32 * 16;
 
 struct AttnParams {
   const __nv_bfloat16* q;
@@ -245,68 +279,425 @@ struct AttnParams {
   Map m;
   const int* slot;
   const int* seqlen;
-  int B, Hq, window;
-  float scale, softcap;
+  int* counters;  // [segments], zero between calls
+  float* parts;   // [CTAs][2][kPartFloats]
+  int B, Hq, G, hg, window;  // G: query heads of a KV head; hg: groups of eight of them
+  float scale_log2, cap_in, cap_out;  // cap_in = scale / softcap, cap_out = softcap * log2 e
   int* status;
 };
 
-// One CTA of 128 threads for each (sequence, query head): 128 keys at a time, a
-// thread a key for the logits, a thread a dimension for the sum, running
-// maximum and sum in fp32.
-__global__ void __launch_bounds__(128) attn_kernel(AttnParams p) {
-  __shared__ float sq[128], sp[128], red[4];
-  __shared__ int64_t srow[128];
-  const int b = blockIdx.y, h = blockIdx.x, tid = threadIdx.x;
-  const int D = p.m.D, hk = h / (p.Hq / p.m.Hkv);
+__device__ __forceinline__ uint4 ld_stream16(const void* p) {
+  uint4 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
+  return v;
+}
+__device__ __forceinline__ uint2 ld_stream8(const void* p) {
+  uint2 v;
+  asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
+  return v;
+}
+// fp16 pair of two biased codes: bytes (sel) of w become 1024 + u, minus 1152
+template <int kSel>
+__device__ __forceinline__ uint32_t half2_of(uint32_t w) {
+  uint32_t x = __byte_perm(w, 0x64646464u, kSel), r;
+  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x64806480u));
+  return r;
+}
+__device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
+  asm volatile(
+      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
+      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
+  uint32_t r;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
+  return r;
+}
+__device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
+  __half2 h = __floats2half2_rn(lo, hi);
+  return *reinterpret_cast<uint32_t*>(&h);
+}
+
+// Blocks [first, first + count) that sequence b attends to.
+__device__ __forceinline__ void blocks_of(const AttnParams& p, int b, int& len, int& lo, int& first, int& count) {
   const int slot = p.slot[b];
-  const int len = slot < 0 ? 0 : min(max(p.seqlen[b], 0), p.m.cols << p.m.shift);
-  const int first = p.window > 0 ? max(0, len - p.window) : 0;
-  if (tid < D) sq[tid] = __bfloat162float(p.q[(int64_t)b * p.q_rs + (int64_t)h * D + tid]);
-  float mx = -INFINITY, sum = 0.f, acc = 0.f;
-  for (int k0 = first; k0 < len; k0 += 128) {
-    const int t = k0 + tid;
-    float x = -INFINITY;
-    int64_t row = -1;
-    __syncthreads();
-    if (t < len) {
-      const int page = page_of(p.m, slot, t, p.status);
-      if (page >= 0) {
-        const int r = t & ((1 << p.m.shift) - 1);
-        row = (((int64_t)page * p.m.Hkv + hk) << p.m.shift) + r;
-        const uint32_t* kc = reinterpret_cast<const uint32_t*>(p.k.codes + row * D);
-        float d = 0.f;
-        for (int i = 0; i < D / 4; ++i) {
-          const uint32_t w = kc[i];
+  len = p.seqlen[b];
+  if (slot >= p.m.rows || len > (p.m.cols << p.m.shift)) atomicExch(p.status, kStatusKvRange);
+  len = (unsigned)slot < (unsigned)p.m.rows ? min(max(len, 0), p.m.cols << p.m.shift) : 0;
+  lo = p.window > 0 ? max(0, len - p.window) : 0;
+  first = lo >> 4;
+  count = len > 0 ? ((len + kBlock - 1) >> 4) - first : 0;
+}
+
+template <int D, bool CAP>
+__global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
+  constexpr int kKs = D / 16;   // k steps of S, m tiles of O
+  constexpr int kKl = D / 64;   // 16-byte loads of a key's row by a quad
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* s_o = reinterpret_cast<float*>(smem);
+  float* s_m = s_o + kWarps * 8 * 128;  // [warps][8]
+  float* s_l = s_m + kWarps * 8;
+  int4* s_rec = reinterpret_cast<int4*>(s_l + kWarps * 8) + (threadIdx.x >> 5) * 32;  // this warp's
+  int* s_pre = reinterpret_cast<int*>(smem + kSmemFixed);  // [B + 1] steps before each sequence (one KV head)
+  __shared__ int s_warp[kWarps], s_flag;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int r = lane >> 2, t = lane & 3;
+  const int V = p.m.Hkv * p.hg;
+
+  // prefix of the steps (kWarps blocks) of every sequence
+  int carry = 0;
+  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+    int n = 0;
+    if (b0 + tid < p.B) {
+      int len, lo, first, count;
+      blocks_of(p, b0 + tid, len, lo, first, count);
+      n = (count + kWarps - 1) / kWarps;
+    }
+    int x = n;
 #pragma unroll
-          for (int e = 0; e < 4; ++e) d += sq[4 * i + e] * code_of(w, e);
+    for (int o = 1; o < 32; o <<= 1) {
+      const int y = __shfl_up_sync(0xffffffffu, x, o);
+      if (lane >= o) x += y;
+    }
+    if (lane == 31) s_warp[warp] = x;
+    __syncthreads();
+    int before = carry;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      if (w < warp) before += s_warp[w];
+      carry += s_warp[w];
+    }
+    if (b0 + tid < p.B) s_pre[b0 + tid] = before + x - n;
+    __syncthreads();
+  }
+  if (tid == 0) s_pre[p.B] = carry;
+  // sequences without a key: zero rows, written by the last CTAs (they have the least to do)
+  for (int b = gridDim.x - 1 - blockIdx.x; b < p.B; b += gridDim.x) {
+    int len, lo, first, count;
+    blocks_of(p, b, len, lo, first, count);
+    if (count == 0)
+      for (int i = tid; i < p.Hq * D / 8; i += kThreads)
+        *reinterpret_cast<uint4*>(p.out + (int64_t)b * p.o_rs + i * 8) = make_uint4(0, 0, 0, 0);
+  }
+  const int64_t total = (int64_t)carry * V;
+  const int64_t per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kMinSteps);
+  int64_t at = blockIdx.x * per;
+  const int64_t end = min(total, at + per);
+  if (at >= end) return;
+  __syncthreads();
+  int b = 0;
+  {  // the last sequence that starts at or before `at` and is not empty
+    int hi = p.B;
+    while (hi - b > 1) {
+      const int mid = (b + hi) >> 1;
+      if ((int64_t)s_pre[mid] * V <= at) b = mid; else hi = mid;
+    }
+  }
+  while (at < end) {
+    while (s_pre[b + 1] == s_pre[b] || (int64_t)s_pre[b + 1] * V <= at) ++b;
+    const int steps = s_pre[b + 1] - s_pre[b];
+    const int64_t off = at - (int64_t)s_pre[b] * V;
+    const int v = (int)(off / steps), st0 = (int)(off % steps);
+    const int st1 = (int)min((int64_t)steps, st0 + (end - at));
+    const int hk = v / p.hg, h0 = hk * p.G + (v % p.hg) * 8;
+    const int heads = min(8, p.G - (v % p.hg) * 8);
+    int len, lo, first, count;
+    blocks_of(p, b, len, lo, first, count);
+    const int slot = p.slot[b];
+    const int blk0 = first + st0 * kWarps + warp;              // this warp's blocks: blk0, blk0 + kWarps, ...
+    const int blk1 = min(first + count, first + st1 * kWarps);
+    const int n_blk = blk1 > blk0 ? (blk1 - blk0 + kWarps - 1) / kWarps : 0;
+
+    // q as the B operand: head r, dims 16 t .. of each 64
+    uint32_t qb[kKs][2];
+    float fac0, fac1;
+    {
+      const bool ok = r < heads;
+      const __nv_bfloat16* qr = p.q + (int64_t)b * p.q_rs + (int64_t)(h0 + (ok ? r : 0)) * D + t * 16;
+      float f[kKs * 4];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < kKl; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float e8[8];
+          dec::unpack8(*reinterpret_cast<const uint4*>(qr + i * 64 + j * 8), e8);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f[i * 16 + j * 8 + e] = ok ? e8[e] : 0.f;
+            top = max(top, __float_as_uint(f[i * 16 + j * 8 + e]) & 0x7fffffffu);
+          }
         }
-        x = d * p.k.scale[row >> 4] * p.scale;
-        if (p.softcap > 0.f) x = p.softcap * tanhf(x / p.softcap);
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int k = top == 0 || top >= 0x7f800000u ? 0 : 13 + 127 - (int)(top >> 23);  // largest |q| into [2^13, 2^14)
+      k = min(k, 100);
+      const float up = __uint_as_float((uint32_t)(127 + k) << 23), down = __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+      for (int i = 0; i < kKs; ++i) {
+        qb[i][0] = pack_f16(f[4 * i] * up, f[4 * i + 1] * up);
+        qb[i][1] = pack_f16(f[4 * i + 2] * up, f[4 * i + 3] * up);
+      }
+      const float fac = (CAP ? p.cap_in : p.scale_log2) * down;
+      fac0 = __shfl_sync(0xffffffffu, fac, 8 * t);  // heads 2 t and 2 t + 1
+      fac1 = __shfl_sync(0xffffffffu, fac, 8 * t + 4);
+    }
+    float o[kKs][4];
+#pragma unroll
+    for (int i = 0; i < kKs; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+    uint4 kr[2 * kKl];   // rows r and r + 8
+    uint4 vr[4];         // rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (D = 64: the low half of each)
+    const uint32_t koff = (uint32_t)(r * D + t * 16), voff = (uint32_t)(2 * t * D + r * (D / 8));
+    auto block_base = [&](int page, int blk) {
+      return code_offset(p.m, page, hk, (blk << 4) & ((1 << p.m.shift) - 1));
+    };
+    auto load_k = [&](int64_t base) {
+      const uint8_t* c = p.k.codes + base + koff;
+#pragma unroll
+      for (int i = 0; i < kKl; ++i) {
+        kr[i] = ld_stream16(c + i * 64);
+        kr[kKl + i] = ld_stream16(c + 8 * D + i * 64);
+      }
+    };
+    auto load_v = [&](int64_t base) {
+      const uint8_t* c = p.v.codes + base + voff;
+#pragma unroll
+      for (int i = 0; i < 4; ++i) {
+        const uint8_t* a = c + ((i & 1) + (i >> 1) * 8) * D;
+        if constexpr (D == 128) {
+          vr[i] = ld_stream16(a);
+        } else {
+          const uint2 h = ld_stream8(a);
+          vr[i].x = h.x;
+          vr[i].y = h.y;
+        }
+      }
+    };
+    for (int i0 = 0; i0 < n_blk; i0 += 32) {
+      const int nb = min(32, n_blk - i0);
+      // records of this warp's next 32 blocks: page, key scale, log2 and inverse of the value scale
+      __syncwarp();
+      if (lane < nb) {
+        const int pos = (blk0 + (i0 + lane) * kWarps) << 4;
+        const int page = page_of(p.m, slot, pos, p.status);
+        float ks = 0.f, lv = -INFINITY, inv = 0.f;  // an unusable page: weights of zero
+        if (page >= 0) {
+          const int64_t so = scale_offset(p.m, page, hk, pos & ((1 << p.m.shift) - 1));
+          ks = p.k.scale[so];
+          float vs = p.v.scale[so];
+          vs = vs < 6.2e-33f ? 6.2e-33f : vs;  // (a NaN stays)
+          lv = log2f(vs);
+          inv = 1.f / vs;
+        }
+        s_rec[lane] = make_int4(max(page, 0), __float_as_int(ks), __float_as_int(lv), __float_as_int(inv));
+      }
+      __syncwarp();
+      int64_t base = block_base(s_rec[0].x, blk0 + i0 * kWarps);
+      load_k(base);
+      load_v(base);
+      for (int i = 0; i < nb; ++i) {
+        const int4 rec = s_rec[i];
+        const int pos = (blk0 + (i0 + i) * kWarps) << 4;
+        const int nx = min(i + 1, nb - 1);
+        base = block_base(s_rec[nx].x, blk0 + (i0 + nx) * kWarps);
+        float c[4] = {0.f, 0.f, 0.f, 0.f};
+#pragma unroll
+        for (int j = 0; j < kKl; ++j) {
+          const uint32_t wl[4] = {kr[j].x, kr[j].y, kr[j].z, kr[j].w};
+          const uint32_t wh[4] = {kr[kKl + j].x, kr[kKl + j].y, kr[kKl + j].z, kr[kKl + j].w};
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const uint32_t a[4] = {half2_of<0x4140>(wl[e]), half2_of<0x4140>(wh[e]), half2_of<0x4342>(wl[e]),
+                                   half2_of<0x4342>(wh[e])};
+            mma_f16(c, a, qb[4 * j + e][0], qb[4 * j + e][1]);
+          }
+        }
+        if (i + 1 < nb) load_k(base);  // in flight behind the rest of this block
+        const float ks = __int_as_float(rec.y), lv = __int_as_float(rec.z), inv = __int_as_float(rec.w);
+        const float f0 = fac0 * ks, f1 = fac1 * ks;
+        float x[4] = {c[0] * f0, c[1] * f1, c[2] * f0, c[3] * f1};  // keys r, r, r + 8, r + 8; heads 2 t, 2 t + 1
+        if constexpr (CAP) {
+#pragma unroll
+          for (int e = 0; e < 4; ++e) x[e] = p.cap_out * tanhf(x[e]);
+        }
+        if (pos < lo || pos + kBlock > len) {
+          const bool a = pos + r >= lo && pos + r < len, bb = pos + r + 8 >= lo && pos + r + 8 < len;
+          x[0] = a ? x[0] : -INFINITY;
+          x[1] = a ? x[1] : -INFINITY;
+          x[2] = bb ? x[2] : -INFINITY;
+          x[3] = bb ? x[3] : -INFINITY;
+        }
+        // M covers x + log2 s_v; scales below 2^-60 count as 2^-60, so that l (the sum of 2^(x - M)) stays in range
+        const float lm = fmaxf(lv, -60.f);
+        float n0 = fmaxf(x[0], x[2]) + lm, n1 = fmaxf(x[1], x[3]) + lm;
+        if (__any_sync(0xffffffffu, n0 > m0 + 4.f || n1 > m1 + 4.f)) {
+#pragma unroll
+          for (int s = 4; s < 32; s <<= 1) {
+            n0 = fmaxf(n0, __shfl_xor_sync(0xffffffffu, n0, s));
+            n1 = fmaxf(n1, __shfl_xor_sync(0xffffffffu, n1, s));
+          }
+          n0 = fmaxf(n0, m0);
+          n1 = fmaxf(n1, m1);
+          const float a0 = n0 == -INFINITY ? 1.f : exp2f(m0 - n0), a1 = n1 == -INFINITY ? 1.f : exp2f(m1 - n1);
+          m0 = n0;
+          m1 = n1;
+          l0 *= a0;
+          l1 *= a1;
+#pragma unroll
+          for (int k = 0; k < kKs; ++k) {
+            o[k][0] *= a0;
+            o[k][1] *= a1;
+            o[k][2] *= a0;
+            o[k][3] *= a1;
+          }
+        }
+        const float d0 = lv + kWeightBits - (m0 == -INFINITY ? 0.f : m0);
+        const float d1 = lv + kWeightBits - (m1 == -INFINITY ? 0.f : m1);
+        const float w0 = exp2f(x[0] + d0), w1 = exp2f(x[1] + d1), w2 = exp2f(x[2] + d0), w3 = exp2f(x[3] + d1);
+        l0 = fmaf(w0 + w2, inv, l0);
+        l1 = fmaf(w1 + w3, inv, l1);
+        const uint32_t pb0 = transpose8x8(pack_f16(w0, w1)), pb1 = transpose8x8(pack_f16(w2, w3));
+#pragma unroll
+        for (int j = 0; j < D / 32; ++j) {
+          const uint32_t wa = j == 0 ? vr[0].x : j == 1 ? vr[0].y : j == 2 ? vr[0].z : vr[0].w;
+          const uint32_t wb = j == 0 ? vr[1].x : j == 1 ? vr[1].y : j == 2 ? vr[1].z : vr[1].w;
+          const uint32_t wc = j == 0 ? vr[2].x : j == 1 ? vr[2].y : j == 2 ? vr[2].z : vr[2].w;
+          const uint32_t wd = j == 0 ? vr[3].x : j == 1 ? vr[3].y : j == 2 ? vr[3].z : vr[3].w;
+#pragma unroll
+          for (int e = 0; e < 2; ++e) {  // dims (D / 8) r + 4 j + 2 e (rows r) and the next (rows r + 8)
+            const uint32_t ab = __byte_perm(wa, wb, e ? 0x7362 : 0x5140), cd = __byte_perm(wc, wd, e ? 0x7362 : 0x5140);
+            const uint32_t a[4] = {half2_of<0x4140>(ab), half2_of<0x4342>(ab), half2_of<0x4140>(cd), half2_of<0x4342>(cd)};
+            mma_f16(o[2 * j + e], a, pb0, pb1);
+          }
+        }
+        if (i + 1 < nb) load_v(base);
       }
     }
-    float m = warp_max(x);
-    if ((tid & 31) == 0) red[tid >> 5] = m;
+    // join the warps: o[k][0], [2] are dims (D / 8) r + 2 k and + 1 of head 2 t; [1], [3] of head 2 t + 1
+#pragma unroll
+    for (int s = 4; s < 32; s <<= 1) {
+      l0 += __shfl_xor_sync(0xffffffffu, l0, s);
+      l1 += __shfl_xor_sync(0xffffffffu, l1, s);
+    }
+    if (r == 0) {
+      s_m[warp * 8 + 2 * t] = m0;
+      s_m[warp * 8 + 2 * t + 1] = m1;
+      s_l[warp * 8 + 2 * t] = l0;
+      s_l[warp * 8 + 2 * t + 1] = l1;
+    }
+#pragma unroll
+    for (int k = 0; k < kKs; ++k) {
+      float* d = s_o + (warp * 8 + 2 * t) * D + (D / 8) * r + 2 * k;
+      *reinterpret_cast<float2*>(d) = make_float2(o[k][0], o[k][2]);
+      *reinterpret_cast<float2*>(d + D) = make_float2(o[k][1], o[k][3]);
+    }
     __syncthreads();
-    m = fmaxf(fmaxf(red[0], red[1]), fmaxf(red[2], red[3]));
-    const float mn = fmaxf(mx, m), base = mn == -INFINITY ? 0.f : mn;
-    const float alpha = exp2f((mx - base) * kLog2e);
-    const float e = exp2f((x - base) * kLog2e);
-    sp[tid] = e;
-    srow[tid] = row;
-    float s = warp_sum(e);
-    __syncthreads();
-    if ((tid & 31) == 0) red[tid >> 5] = s;
-    __syncthreads();
-    sum = sum * alpha + (red[0] + red[1] + red[2] + red[3]);
-    acc *= alpha;
-    mx = mn;
-    if (tid < D)
-      for (int i = 0; i < min(128, len - k0); ++i) {
-        const int64_t r = srow[i];
-        if (r >= 0) acc += sp[i] * (p.v.scale[r >> 4] * (float)((int)p.v.codes[r * D + tid] - 128));
+    const bool whole = st0 == 0 && st1 == steps;
+    const int64_t seg0 = (int64_t)s_pre[b] * V + (int64_t)v * steps;  // the segment's first step
+    const int64_t cta0 = seg0 / per;
+    float* part = p.parts + ((int64_t)blockIdx.x * 2 + (cta0 == blockIdx.x ? 1 : 0)) * kPartFloats;
+    constexpr int kPer = 8 * D / kThreads;  // consecutive dims of one head for each thread
+    {
+      const int g = tid * kPer / D, d = tid * kPer % D;
+      float mm = -INFINITY;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w * 8 + g]);
+      float ll = 0.f, acc[kPer];
+#pragma unroll
+      for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float mw = s_m[w * 8 + g];
+        const float f = mw == -INFINITY ? (s_l[w * 8 + g] == 0.f ? 0.f : 1.f) : exp2f(mw - mm);  // l is 0 or NaN
+        ll += f * s_l[w * 8 + g];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) acc[e] += f * s_o[(w * 8 + g) * D + d + e];
       }
+      if (whole) {
+        if (g < heads) {
+          const float inv = ll == 0.f ? 0.f : 1.f / ll;
+          __nv_bfloat16* y = p.out + (int64_t)b * p.o_rs + (int64_t)(h0 + g) * D + d;
+#pragma unroll
+          for (int e = 0; e < kPer; e += 2)
+            *reinterpret_cast<uint32_t*>(y + e) = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
+        }
+      } else {
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) part[g * D + d + e] = acc[e];
+        if (d == 0) {
+          part[8 * D + g] = mm;
+          part[8 * D + 8 + g] = ll;
+        }
+      }
+    }
+    if (!whole) {
+      const int64_t cta1 = (seg0 + steps - 1) / per;
+      const int np = (int)(cta1 - cta0) + 1;
+      __threadfence();
+      __syncthreads();
+      if (tid == 0) s_flag = atomicAdd(p.counters + b * V + v, 1) == np - 1;
+      __syncthreads();
+      if (s_flag) {
+        __threadfence();
+        auto part_of = [&](int i) { return p.parts + ((cta0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats; };
+        {  // warp g: the parts' weights for head g, 2^(M_i - M) / l
+          const int g = warp;
+          float* wgt = s_o + g * kMaxCtas;
+          float mm = -INFINITY;
+          for (int i = lane; i < np; i += 32) mm = fmaxf(mm, __ldcg(part_of(i) + 8 * D + g));
+          mm = warp_max(mm);
+          float ll = 0.f;
+          for (int i = lane; i < np; i += 32) {
+            const float mi = __ldcg(part_of(i) + 8 * D + g), li = __ldcg(part_of(i) + 8 * D + 8 + g);
+            const float f = mi == -INFINITY ? (li == 0.f ? 0.f : 1.f) : exp2f(mi - mm);
+            wgt[i] = f;
+            ll += f * li;
+          }
+          ll = warp_sum(ll);
+          __syncwarp();
+          for (int i = lane; i < np; i += 32) wgt[i] *= ll == 0.f ? 0.f : 1.f / ll;
+        }
+        __syncthreads();
+        const int g = tid * kPer / D, d = tid * kPer % D;
+        const float* wgt = s_o + g * kMaxCtas;
+        float acc[kPer];
+#pragma unroll
+        for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+        for (int i0 = 0; i0 < np; i0 += 8) {
+          float x[8][kPer];
+#pragma unroll
+          for (int i = 0; i < 8; ++i) {
+            const float* src = part_of(min(i0 + i, np - 1)) + g * D + d;
+            if constexpr (kPer == 4) {
+              const float4 q4 = __ldcg(reinterpret_cast<const float4*>(src));
+              x[i][0] = q4.x, x[i][1] = q4.y, x[i][2] = q4.z, x[i][3] = q4.w;
+            } else {
+              const float2 q2 = __ldcg(reinterpret_cast<const float2*>(src));
+              x[i][0] = q2.x, x[i][1] = q2.y;
+            }
+          }
+#pragma unroll
+          for (int i = 0; i < 8; ++i)
+            if (i0 + i < np) {
+#pragma unroll
+              for (int e = 0; e < kPer; ++e) acc[e] += wgt[i0 + i] * x[i][e];
+            }
+        }
+        if (g < heads) {
+          __nv_bfloat16* y = p.out + (int64_t)b * p.o_rs + (int64_t)(h0 + g) * D + d;
+#pragma unroll
+          for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(y + e) = pack_bf16(acc[e], acc[e + 1]);
+        }
+        if (tid == 0) p.counters[b * V + v] = 0;  // ready for the next call
+      }
+    }
+    __syncthreads();  // the sums are free again
+    at += st1 - st0;
   }
-  if (tid < D) p.out[(int64_t)b * p.o_rs + (int64_t)h * D + tid] = __float2bfloat16(sum == 0.f ? 0.f : acc / sum);
 }
 
 // ------------------------------------------------------------------ host
@@ -316,7 +707,7 @@ static void check_pool(const at::Tensor& codes, const at::Tensor& scale, const a
   const int64_t P = codes.size(2), D = codes.size(3);
   TORCH_CHECK(P >= kBlock && (P & (P - 1)) == 0 && P <= 65536, what, ": page is a power of two of at least 16");
   TORCH_CHECK(D == 64 || D == 128, what, ": head_dim 64 or 128");
-  TORCH_CHECK(codes.size(0) < (int64_t(1) << 31) && codes.size(1) >= 1, what, ": pages and KV heads");
+  TORCH_CHECK(codes.size(0) >= 1 && codes.size(0) < (int64_t(1) << 31) && codes.size(1) >= 1, what, ": pages and KV heads");
   TORCH_CHECK(scale.device() == codes.device() && scale.scalar_type() == at::kFloat && scale.dim() == 3 &&
                   scale.is_contiguous() && scale.size(0) == codes.size(0) && scale.size(1) == codes.size(1) &&
                   scale.size(2) == P / kBlock,
@@ -438,7 +829,7 @@ void gather_kv8(at::Tensor codes, at::Tensor scale, at::Tensor page_table, at::T
 
 void kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor vc, at::Tensor vs,
                           at::Tensor page_table, at::Tensor slot, at::Tensor seqlen, at::Tensor out, int64_t Hq,
-                          double scale, int64_t window, double softcap) {
+                          double scale, at::Tensor workspace, int64_t window, double softcap) {
   using namespace kv8;
   check_pool(kc, ks, page_table, "kv8_decode_attention");
   check_pool(vc, vs, page_table, "kv8_decode_attention");
@@ -453,7 +844,12 @@ void kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor
   check_ints(slot, kc, B, "kv8_decode_attention: slot [B]");
   check_ints(seqlen, kc, B, "kv8_decode_attention: seqlen [B]");
   TORCH_CHECK(window >= 0 && window < (int64_t(1) << 31) && softcap >= 0, "kv8_decode_attention: window and softcap");
-  TORCH_CHECK(B <= 65535, "kv8_decode_attention: at most 65535 sequences");
+  const int64_t G = Hq / Hkv, hg = (G + 7) / 8;
+  TORCH_CHECK(B <= kMaxSeqs && B * Hkv * hg <= kMaxSegments,
+              "kv8_decode_attention: at most 8192 sequences and 65536 (sequence, KV head, eight query heads)");
+  TORCH_CHECK(workspace.device() == kc.device() && workspace.scalar_type() == at::kByte && workspace.is_contiguous() &&
+                  workspace.numel() >= kWorkspaceBytes && reinterpret_cast<uintptr_t>(workspace.data_ptr()) % 16 == 0,
+              "kv8_decode_attention: workspace from kv8_workspace on the cache's device");
   if (B == 0) return;
   c10::cuda::CUDAGuard g(kc.device());
   AttnParams p{};
@@ -466,14 +862,44 @@ void kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor
   p.m = make_map(kc, page_table);
   p.slot = slot.data_ptr<int>();
   p.seqlen = seqlen.data_ptr<int>();
+  p.counters = reinterpret_cast<int*>(workspace.data_ptr());
+  p.parts = reinterpret_cast<float*>(p.counters + kMaxSegments);
   p.B = (int)B;
   p.Hq = (int)Hq;
+  p.G = (int)G;
+  p.hg = (int)hg;
   p.window = (int)window;
-  p.scale = (float)scale;
-  p.softcap = (float)softcap;
+  p.scale_log2 = (float)scale * kLog2e;
+  if (softcap > 0) {
+    p.cap_in = (float)(scale / softcap);
+    p.cap_out = (float)softcap * kLog2e;
+  }
   p.status = device_status_word();
-  attn_kernel<<<dim3((unsigned)Hq, (unsigned)B), 128, 0, at::cuda::getCurrentCUDAStream()>>>(p);
-  AETHER_CUDA_CHECK(cudaGetLastError());
+  int64_t keys = (int64_t)p.m.cols << p.m.shift;
+  if (window > 0) keys = std::min<int64_t>(keys, window + kBlock);
+  const int64_t most = B * Hkv * hg * std::max<int64_t>(1, (keys + kWarps * kBlock - 1) / (kWarps * kBlock));
+  const int grid = (int)std::min<int64_t>(std::min(2 * num_sms(current_device()), kMaxCtas), most);
+  const int smem = kSmemFixed + ((int)B + 1) * 4;
+  auto st = at::cuda::getCurrentCUDAStream();
+  auto launch = [&](auto kernel, bool* set) {
+    const int dev = current_device();
+    if (!set[dev]) {
+      AETHER_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
+                                             kSmemFixed + (kMaxSeqs + 1) * 4));
+      set[dev] = true;
+    }
+    kernel<<<grid, kThreads, smem, st>>>(p);
+    AETHER_CUDA_CHECK(cudaGetLastError());
+  };
+  static bool set[4][64] = {};
+  if (D == 128 && softcap > 0)
+    launch(attn_kernel<128, true>, set[0]);
+  else if (D == 128)
+    launch(attn_kernel<128, false>, set[1]);
+  else if (softcap > 0)
+    launch(attn_kernel<64, true>, set[2]);
+  else
+    launch(attn_kernel<64, false>, set[3]);
 }
 
 }  // namespace aether
