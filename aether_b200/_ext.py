@@ -35,22 +35,20 @@ class _CountingModule:
         self._mod = mod
         self.enabled = False
         self.launches = 0
-        self._cache = {}
 
     def __getattr__(self, name):
         fn = getattr(self._mod, name)
         if not callable(fn):
             return fn
-        if name not in self._cache:
-            k = _KERNELS_PER_CALL.get(name, 1)
+        k = _KERNELS_PER_CALL.get(name, 1)
 
-            def wrapped(*a, _fn=fn, _k=k, **kw):
-                if self.enabled:
-                    self.launches += _k
-                return _fn(*a, **kw)
+        def wrapped(*a, _fn=fn, _k=k, **kw):
+            if self.enabled:
+                self.launches += _k
+            return _fn(*a, **kw)
 
-            self._cache[name] = wrapped
-        return self._cache[name]
+        setattr(self, name, wrapped)  # found without this method from now on
+        return wrapped
 
 
 _PROXY = _CountingModule(_C) if _C is not None else None

@@ -838,14 +838,12 @@ def gather_kv8(codes, scale, page_table, slot, first, n, out=None):
     """bf16 [B, n, Hkv, D]: positions first .. first + n (``first`` an int for all
     or int32 [B]) of page-table rows slot [B] of an 8-bit pool. Positions that
     the table does not reach read as zero."""
-    if out is None:
-        out = torch.empty(slot.shape[0], n, codes.shape[1], codes.shape[3], dtype=BF16, device=codes.device)
     if _cuda(codes):
         if isinstance(first, torch.Tensor):
-            C().gather_kv8(codes, scale, page_table, slot, first, 0, out)
-        else:
-            C().gather_kv8(codes, scale, page_table, slot, None, first, out)
-        return out
+            return C().gather_kv8(codes, scale, page_table, slot, first, 0, n, out)
+        return C().gather_kv8(codes, scale, page_table, slot, None, first, n, out)
+    if out is None:
+        out = torch.empty(slot.shape[0], n, codes.shape[1], codes.shape[3], dtype=BF16)
     for b in range(slot.shape[0]):
         f = int(first[b]) if isinstance(first, torch.Tensor) else int(first)
         v = ref.kv8_values(codes, scale, page_table[int(slot[b])], f + n)[f:]
@@ -862,15 +860,15 @@ def kv8_decode_attention(q, kc, ks, vc, vs, page_table, slot, seqlen, Hq, scale,
     > 0: the last ``window`` keys; ``softcap`` > 0: soft-capped logits.
     ``workspace``: from ``kv8_workspace``, kept by the caller (a captured graph
     must be given one); None allocates it."""
-    if out is None:
-        out = torch.empty(q.shape[0], Hq * kc.shape[3], dtype=BF16, device=q.device)
     if _cuda(q):
         if workspace is None:
             workspace = kv8_workspace(q.device)
-        C().kv8_decode_attention(q, kc, ks, vc, vs, page_table, slot, seqlen, out, Hq, scale, workspace, window, softcap)
-        return out
+        return C().kv8_decode_attention(q, kc, ks, vc, vs, page_table, slot, seqlen, out, Hq, scale, workspace, window,
+                                        softcap)
     _kv8_rows(q, "kv8_decode_attention: q")
     D = kc.shape[3]
+    if out is None:
+        out = torch.empty(q.shape[0], Hq * D, dtype=BF16)
     for b in range(q.shape[0]):
         L, s = int(seqlen[b]), int(slot[b])
         if L <= 0 or s < 0:
@@ -951,12 +949,12 @@ def linear_w4(x, w, bias=None, residual=None, swiglu=False, out=None):
     rows the 4-bit weights are multiplied as they are (exact codes, fp32 sums and
     scales); more rows expand them to bf16 for the tensor-core GEMM."""
     M = x.shape[0]
+    if M <= W4_ROWS and _cuda(x):
+        return C().linear_w4(x, w.q, w.s, w.N, w.K, w.group, bias, residual, swiglu, out)
     if out is None:
         out = torch.empty(M, w.N // 2 if swiglu else w.N, dtype=BF16, device=x.device)
     if _cuda(x):
-        if M <= W4_ROWS:
-            C().linear_w4(x, w.q, w.s, w.N, w.K, w.group, bias, residual, swiglu, out)
-        elif w.N % 8 == 0 and out.shape[1] % 8 == 0:
+        if w.N % 8 == 0 and out.shape[1] % 8 == 0:
             wb = dequant_w4(w)
             if swiglu:
                 out.copy_(swiglu_residual(gemm(x, wb, bias=bias), residual))

@@ -11,6 +11,11 @@ once on its own:
     python -m aether_b200.profile_cases skinny      # decode GEMM 1 x 3584 -> 37888 (Qwen-7B gate/up)
     python -m aether_b200.profile_cases decode_attn # split-K decode attention B8 Hq28 Hkv4 S8192
     python -m aether_b200.profile_cases decode_attn_b1  # the same at batch 1, 2048 keys, 32 splits
+    python -m aether_b200.profile_cases kv8_attn    # attention over an 8-bit paged cache, B64 Hq28 Hkv4 S4096
+    python -m aether_b200.profile_cases kv8_append  # RoPE + 8-bit quantisation + append, 8 sequences x 2048 tokens
+    python -m aether_b200.profile_cases w4          # 4-bit weights: 1 x 3584 -> 37888 (SwiGLU)
+    python -m aether_b200.profile_cases w4_b16      # 4-bit weights: 16 x 18944 -> 3584
+    python -m aether_b200.profile_cases w4_b64      # 4-bit weights: 64 x 3584 -> 37888 (SwiGLU)
     python -m aether_b200.profile_cases adamw       # fused AdamW over 64M fp32 params
     python -m aether_b200.profile_cases decode7b    # eager Qwen2.5-7B-shape decode steps (batch 1, 2048 cached)
                                                     # inside NVTX range "decode": for the launch list only
@@ -90,6 +95,61 @@ def decode_attn_b1(reps):
     counters = torch.zeros(Hkv, dtype=torch.int32, device="cuda")
     for _ in range(reps):
         F.decode_attention(q, kc, vc, slot, seqlen, out, Hq, D ** -0.5, splits=32, counters=counters)
+
+
+def _kv8_pool(pages, Hkv, P, D):
+    return (torch.randint(1, 256, (pages, Hkv, P, D), dtype=torch.uint8, device="cuda"),
+            torch.rand(pages, Hkv, P // 16, device="cuda") * 0.03)
+
+
+def kv8_attn(reps):
+    B, Hq, Hkv, D, P, S = 64, 28, 4, 128, 64, 4096
+    n = B * S // P
+    kc, ks = _kv8_pool(n, Hkv, P, D)
+    vc, vs = _kv8_pool(n, Hkv, P, D)
+    table = torch.randperm(n, device="cuda").int().view(B, -1)
+    q = torch.randn(B, Hq * D, device="cuda").bfloat16()
+    slot = torch.arange(B, dtype=torch.int32, device="cuda")
+    seqlen = torch.full((B,), S, dtype=torch.int32, device="cuda")
+    ws = F.kv8_workspace("cuda")
+    for _ in range(reps):
+        F.kv8_decode_attention(q, kc, ks, vc, vs, table, slot, seqlen, Hq, D ** -0.5, workspace=ws)
+
+
+def kv8_append(reps):
+    B, Hq, Hkv, D, P, S = 8, 28, 4, 128, 64, 2048
+    n = B * S // P
+    kc, ks = _kv8_pool(n, Hkv, P, D)
+    vc, vs = _kv8_pool(n, Hkv, P, D)
+    table = torch.randperm(n, device="cuda").int().view(B, -1)
+    qkv = torch.randn(B * S, (Hq + 2 * Hkv) * D, device="cuda").bfloat16()
+    cos, sin = torch.rand(S, D // 2, device="cuda"), torch.rand(S, D // 2, device="cuda")
+    slot = torch.arange(B, dtype=torch.int32, device="cuda")
+    start = torch.arange(B + 1, dtype=torch.int32, device="cuda") * S
+    for _ in range(reps):
+        F.rope_kv8_append(qkv, torch.zeros_like(slot), slot, cos, sin, kc, ks, vc, vs, table, Hq, row_start=start)
+
+
+def _w4(reps, M, N, K, swiglu):
+    w = F.W4Weight(torch.randint(-(1 << 31), 1 << 31, (N // 16, K // 128, 2, 32, 4), device="cuda").int(),
+                   torch.rand(N // 16, K // 128, 8, 2, device="cuda").half(), N, K, 128)
+    x = torch.randn(M, K, device="cuda").bfloat16()
+    flush = torch.empty(256 << 20, dtype=torch.uint8, device="cuda")
+    for _ in range(reps):
+        flush.zero_()
+        F.linear_w4(x, w, swiglu=swiglu)
+
+
+def w4(reps):
+    _w4(reps, 1, 37888, 3584, True)
+
+
+def w4_b16(reps):
+    _w4(reps, 16, 3584, 18944, False)
+
+
+def w4_b64(reps):
+    _w4(reps, 64, 37888, 3584, True)
 
 
 def adamw(reps):
@@ -230,7 +290,8 @@ def gemm_tp(reps):
         print(f"gemm_tp {tag}: {ms * 1e3:.1f} us per AG-GEMM + GEMM-RS pair, {flops / ms / 1e9:.0f} TFLOP/s")
 
 
-CASES = {f.__name__: f for f in (gemm, attn_fwd, attn_bwd, skinny, decode_attn, decode_attn_b1, adamw, decode7b,
+CASES = {f.__name__: f for f in (gemm, attn_fwd, attn_bwd, skinny, decode_attn, decode_attn_b1, kv8_attn, kv8_append, w4, w4_b16,
+                                 w4_b64, adamw, decode7b,
                                  decode7b_tp8, rows, gemm_tp)}
 
 

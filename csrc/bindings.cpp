@@ -67,14 +67,16 @@ void attention_fwd_tc(at::Tensor q, at::Tensor k, at::Tensor v, at::Tensor out, 
 void rope_kv8_append(at::Tensor qkv, at::Tensor pos, at::Tensor slot, std::optional<at::Tensor> row_start,
                      at::Tensor cos_t, at::Tensor sin_t, at::Tensor kc, at::Tensor ks, at::Tensor vc, at::Tensor vs,
                      at::Tensor page_table, int64_t Hq, at::Tensor out);
-void gather_kv8(at::Tensor codes, at::Tensor scale, at::Tensor page_table, at::Tensor slot,
-                std::optional<at::Tensor> first, int64_t first0, at::Tensor out);
-void kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor vc, at::Tensor vs,
-                          at::Tensor page_table, at::Tensor slot, at::Tensor seqlen, at::Tensor out, int64_t Hq,
-                          double scale, at::Tensor workspace, int64_t window, double softcap);
+at::Tensor gather_kv8(at::Tensor codes, at::Tensor scale, at::Tensor page_table, at::Tensor slot,
+                      std::optional<at::Tensor> first, int64_t first0, int64_t n, std::optional<at::Tensor> into);
+at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor vc, at::Tensor vs,
+                                at::Tensor page_table, at::Tensor slot, at::Tensor seqlen,
+                                std::optional<at::Tensor> into, int64_t Hq, double scale, at::Tensor workspace,
+                                int64_t window, double softcap);
 // w4.cu
-void linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group,
-               std::optional<at::Tensor> bias, std::optional<at::Tensor> residual, bool swiglu, at::Tensor y);
+at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group,
+                     std::optional<at::Tensor> bias, std::optional<at::Tensor> residual, bool swiglu,
+                     std::optional<at::Tensor> out);
 void dequant_w4(at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group, at::Tensor out);
 // gemm_skinny.cu
 void skinny_gemm(at::Tensor x, at::Tensor w, at::Tensor acc, int64_t splits, int64_t acc_mc,

@@ -81,8 +81,8 @@ struct AppendParams {
   int* status;
 };
 
-// A warp owns one (block of 16 positions, head), so a block's scale has one
-// writer and the result depends on no order:
+// A warp owns one (block of 16 positions, head) at a time, so a block's scale
+// has one writer and the result depends on no order:
 //   y = rope(x) (k heads) or x (v heads), each product rounded by itself
 //   s = max(s_old if the block holds older tokens, max |y| / 127)
 //   code = rint(y * (1 / s)); older codes c become rint(c * (s_old / s))
@@ -90,14 +90,21 @@ struct AppendParams {
 // as NaN. With row_start, unit u belongs to the sequence b whose first unit
 // row_start[b] / 16 + 2 b is the last one not after u: a sequence of n rows
 // touches at most n / 16 + 1.875 blocks, so these ranges never overlap.
+// Bound by the bytes of qkv and out: a warp has a block's 4 KB of one head in
+// flight, and the warps of a CTA walk over the heads of one block of tokens, so
+// that its rows of cos and sin come from L1 after the first. A few tokens get a
+// warp for each head instead (one token a block: latency is all there is).
+constexpr int kAppendWarps = 8;
+
 template <int D>
-__global__ void __launch_bounds__(128) append_kernel(AppendParams p) {
+__global__ void __launch_bounds__(kAppendWarps * 32, 3) append_kernel(AppendParams p) {
   constexpr int kLanes = D / 16;            // lanes of one token: 8 + 8 dims each
   constexpr int kTok = 32 / kLanes;         // tokens side by side
   constexpr int kIt = kBlock / kTok;
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int H = p.Hq + 2 * p.m.Hkv;
-  const int h = blockIdx.y * 4 + warp;
   int b, j, r0, n;
   if (p.row_start == nullptr) {
     b = blockIdx.x;
@@ -117,7 +124,6 @@ __global__ void __launch_bounds__(128) append_kernel(AppendParams p) {
     n = p.row_start[b + 1] - r0;
     j = u - ((r0 >> 4) + 2 * b);
   }
-  if (h >= H) return;
   const int pos = p.pos[b], slot = p.slot[b];
   const int base = ((pos >> 4) + j) << 4;  // first position of the block
   const int lo = max(pos, base), hi = min(pos + n, base + kBlock);
@@ -129,109 +135,159 @@ __global__ void __launch_bounds__(128) append_kernel(AppendParams p) {
   const int page = page_of(p.m, slot, base, p.status);
   if (page < 0) return;
   const int c = (lane % kLanes) * 8, sub = lane / kLanes;
-  const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.m.Hkv;
-  float y[kIt][16];
-  uint32_t top = 0;
+  const int row = base & ((1 << p.m.shift) - 1);
+  for (int h = blockIdx.y * kAppendWarps + warp; h < H; h += gridDim.y * kAppendWarps) {
+    const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.m.Hkv;
+    const Pool& pool = is_v ? p.v : p.k;
+    const int hk = h - p.Hq - (is_v ? p.m.Hkv : 0);
+    uint8_t* codes = pool.codes + code_offset(p.m, page, max(hk, 0), row);
+    float* scale = pool.scale + scale_offset(p.m, page, max(hk, 0), row);
+    const float s_old = !is_q && lo > base ? *scale : 0.f;
+    uint4 xa[kIt], xb[kIt];
 #pragma unroll
-  for (int i = 0; i < kIt; ++i) {
-    const int t = base + i * kTok + sub;
-    if (t < lo || t >= hi) continue;
-    const int64_t r = r0 + (t - pos);
-    const __nv_bfloat16* x = p.qkv + r * p.rs + (int64_t)h * D + c;
-    float a[8], bb[8];
-    dec::unpack8(*reinterpret_cast<const uint4*>(x), a);
-    dec::unpack8(*reinterpret_cast<const uint4*>(x + D / 2), bb);
-    if (!is_v) {
-      const float* cp = p.cos_t + (int64_t)t * (D / 2) + c;
-      const float* sp = p.sin_t + (int64_t)t * (D / 2) + c;
+    for (int i = 0; i < kIt; ++i) {
+      const int t = base + i * kTok + sub;
+      if (t >= lo && t < hi) {
+        const __nv_bfloat16* x = p.qkv + (int64_t)(r0 + (t - pos)) * p.rs + (int64_t)h * D + c;
+        xa[i] = *reinterpret_cast<const uint4*>(x);
+        xb[i] = *reinterpret_cast<const uint4*>(x + D / 2);
+      }
+    }
+    // dims c .. and D / 2 + c .. of position t, rotated
+    auto value = [&](int i, int t, float (&a)[8], float (&bb)[8]) {
+      dec::unpack8(xa[i], a);
+      dec::unpack8(xb[i], bb);
+      if (is_v) return;
+      const float4* cp = reinterpret_cast<const float4*>(p.cos_t + (int64_t)t * (D / 2) + c);
+      const float4* sp = reinterpret_cast<const float4*>(p.sin_t + (int64_t)t * (D / 2) + c);
+      const float4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
+      const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
+      const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
         const float x1 = a[e], x2 = bb[e];
-        a[e] = __fsub_rn(__fmul_rn(x1, cp[e]), __fmul_rn(x2, sp[e]));
-        bb[e] = __fadd_rn(__fmul_rn(x2, cp[e]), __fmul_rn(x1, sp[e]));
+        a[e] = __fsub_rn(__fmul_rn(x1, cs[e]), __fmul_rn(x2, sn[e]));
+        bb[e] = __fadd_rn(__fmul_rn(x2, cs[e]), __fmul_rn(x1, sn[e]));
       }
-      __nv_bfloat16* o = p.out + r * p.os + (int64_t)h * D + c;
-      *reinterpret_cast<uint4*>(o) = dec::pack8(a);
-      *reinterpret_cast<uint4*>(o + D / 2) = dec::pack8(bb);
-    }
+    };
+    uint32_t top = 0;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
-      y[i][e] = a[e];
-      y[i][8 + e] = bb[e];
-      top = max(top, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(bb[e]) & 0x7fffffffu));
-    }
-  }
-  if (is_q) return;
-  top = __reduce_max_sync(0xffffffffu, top);
-  const Pool& pool = is_v ? p.v : p.k;
-  const int hk = h - p.Hq - (is_v ? p.m.Hkv : 0);
-  const int row = base & ((1 << p.m.shift) - 1);
-  uint8_t* codes = pool.codes + code_offset(p.m, page, hk, row);
-  float* scale = pool.scale + scale_offset(p.m, page, hk, row);
-  // 2^-100: a block of zeros gets a tiny scale, and 1 / s stays finite
-  const float s_new = __fdiv_rn(__uint_as_float(max(top, 0x0d800000u)), 127.f);
-  float s = s_new;
-  if (lo > base) {
-    const float s_old = *scale;
-    s = __uint_as_float(max(__float_as_uint(s_old), __float_as_uint(s_new)));
-    const float f = __fdiv_rn(s_old, s);
-    for (int i = lane; i < (lo - base) * (D / 4); i += 32) {
-      uint32_t w = reinterpret_cast<uint32_t*>(codes)[i], o = 0;
+    for (int i = 0; i < kIt; ++i) {
+      const int t = base + i * kTok + sub;
+      if (t < lo || t >= hi) continue;
+      float a[8], bb[8];
+      value(i, t, a, bb);
+      if (!is_v) {
+        __nv_bfloat16* o = p.out + (int64_t)(r0 + (t - pos)) * p.os + (int64_t)h * D + c;
+        *reinterpret_cast<uint4*>(o) = dec::pack8(a);
+        *reinterpret_cast<uint4*>(o + D / 2) = dec::pack8(bb);
+      }
+      if (!is_q) {
 #pragma unroll
-      for (int e = 0; e < 4; ++e) o |= (uint32_t)(__float2int_rn(__fmul_rn(code_of(w, e), f)) + 128) << (8 * e);
-      reinterpret_cast<uint32_t*>(codes)[i] = o;
+        for (int e = 0; e < 8; ++e)
+          top = max(top, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(bb[e]) & 0x7fffffffu));
+      }
     }
-  }
-  __syncwarp();
-  if (lane == 0) *scale = s;
-  const float inv = __fdiv_rn(1.f, s);
+    if (is_q) continue;
+    top = __reduce_max_sync(0xffffffffu, top);
+    // 2^-100: a block of zeros gets a tiny scale, and 1 / s stays finite
+    const float s_new = __fdiv_rn(__uint_as_float(max(top, 0x0d800000u)), 127.f);
+    float s = s_new;
+    if (lo > base) {
+      s = __uint_as_float(max(__float_as_uint(s_old), __float_as_uint(s_new)));
+      const float f = __fdiv_rn(s_old, s);
+      if (f != 1.f)  // the scale has grown (or is no number)
+        for (int i = lane; i < (lo - base) * (D / 4); i += 32) {
+          uint32_t w = reinterpret_cast<uint32_t*>(codes)[i], o = 0;
 #pragma unroll
-  for (int i = 0; i < kIt; ++i) {
-    const int t = base + i * kTok + sub;
-    if (t < lo || t >= hi) continue;
-    uint32_t w[4] = {0, 0, 0, 0};
-#pragma unroll
-    for (int e = 0; e < 16; ++e) {
-      const int q = min(127, max(-127, __float2int_rn(__fmul_rn(y[i][e], inv))));
-      w[e >> 2] |= (uint32_t)(q + 128) << (8 * (e & 3));
+          for (int e = 0; e < 4; ++e) o |= (uint32_t)(__float2int_rn(__fmul_rn(code_of(w, e), f)) + 128) << (8 * e);
+          reinterpret_cast<uint32_t*>(codes)[i] = o;
+        }
     }
-    uint8_t* d = codes + (t - base) * D + c;
-    *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
-    *reinterpret_cast<uint2*>(d + D / 2) = make_uint2(w[2], w[3]);
+    __syncwarp();
+    if (lane == 0) *scale = s;
+    const float inv = __fdiv_rn(1.f, s);
+#pragma unroll
+    for (int i = 0; i < kIt; ++i) {
+      const int t = base + i * kTok + sub;
+      if (t < lo || t >= hi) continue;
+      float a[8], bb[8];
+      value(i, t, a, bb);  // again: cheaper than 64 registers to keep it
+      uint32_t w[4] = {0, 0, 0, 0};
+#pragma unroll
+      for (int e = 0; e < 16; ++e) {
+        const int q = min(127, max(-127, __float2int_rn(__fmul_rn(e < 8 ? a[e] : bb[e - 8], inv))));
+        w[e >> 2] |= (uint32_t)(q + 128) << (8 * (e & 3));
+      }
+      uint8_t* d = codes + (t - base) * D + c;
+      *reinterpret_cast<uint2*>(d) = make_uint2(w[0], w[1]);
+      *reinterpret_cast<uint2*>(d + D / 2) = make_uint2(w[2], w[3]);
+    }
   }
 }
 
 // ------------------------------------------------------------------ gather
-// out [B, n, Hkv, D] bf16 = code * scale of positions first[b] .. first[b] + n:
-// a thread turns 16 codes into two 16-byte stores. Bound by the bytes moved.
-__global__ void __launch_bounds__(256) gather_kernel(Pool c, Map m, const int* __restrict__ slot,
-                                                     const int* __restrict__ first, int first0, int64_t n, int64_t total,
-                                                     __nv_bfloat16* __restrict__ out, int* status) {
-  const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
-  if (i >= total) return;
-  const int per = m.D / 16;
-  const int ch = (int)(i % per) * 16;
-  const int64_t r = i / per;  // (b, position, head)
-  const int h = (int)(r % m.Hkv);
-  const int64_t bt = r / m.Hkv;
-  const int b = (int)(bt / n);
-  const int t = (first ? first[b] : first0) + (int)(bt % n);
-  uint4 lo = make_uint4(0, 0, 0, 0), hi = lo;
-  const int page = page_of(m, slot[b], t, status);
-  if (page >= 0) {
-    const int row = t & ((1 << m.shift) - 1);
-    const uint4 w = *reinterpret_cast<const uint4*>(c.codes + code_offset(m, page, h, row) + ch);
-    const float s = c.scale[scale_offset(m, page, h, row)];
-    const uint32_t ws[4] = {w.x, w.y, w.z, w.w};
-    float v[16];
+struct GatherParams {
+  Pool c;
+  Map m;
+  const int* slot;
+  const int* first;  // [B], or null: first0 for all
+  int first0, n, heads;  // heads of one CTA
+  __nv_bfloat16* out;    // [B, n, Hkv, D]
+  int* status;
+};
+
+// out = code * scale, rounded once: a thread keeps its head and its 16 dims and
+// turns kGatherRows positions, all loaded before the first is stored. Bound by
+// the bytes moved; a position's heads are one run of the output, and 128 bytes
+// of a head's row one line of the pool.
+constexpr int kGatherThreads = 256;
+constexpr int kGatherRows = 4;
+
+// four codes of w times s
+__device__ __forceinline__ uint2 four(uint32_t w, float s) {
+  float v[4];
 #pragma unroll
-    for (int e = 0; e < 16; ++e) v[e] = code_of(ws[e >> 2], e & 3) * s;
-    lo = make_uint4(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]), pack_bf16(v[4], v[5]), pack_bf16(v[6], v[7]));
-    hi = make_uint4(pack_bf16(v[8], v[9]), pack_bf16(v[10], v[11]), pack_bf16(v[12], v[13]), pack_bf16(v[14], v[15]));
+  for (int e = 0; e < 4; ++e)  // 2^23 + u, minus 2^23 + 128, exact
+    v[e] = __fmul_rn(__uint_as_float(__byte_perm(w, 0x4b000000u, 0x7650 + e)) - 8388736.f, s);
+  return make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
+}
+
+__global__ void __launch_bounds__(kGatherThreads) gather_kernel(GatherParams p) {
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  const int per = p.m.D / 16;  // threads of a row
+  const int side = kGatherThreads / (per * p.heads);  // positions side by side
+  const int ch = (threadIdx.x % per) * 16, hs = threadIdx.x / per;
+  const int h = blockIdx.z * p.heads + hs % p.heads, sub = hs / p.heads;
+  const int b = blockIdx.y;
+  if (sub >= side || h >= p.m.Hkv) return;
+  const int i0 = blockIdx.x * side * kGatherRows + sub;
+  const int slot = p.slot[b], f = p.first ? p.first[b] : p.first0;
+  int page[kGatherRows];
+#pragma unroll
+  for (int k = 0; k < kGatherRows; ++k) page[k] = i0 + k * side < p.n ? page_of(p.m, slot, f + i0 + k * side, p.status) : -1;
+  uint4 w[kGatherRows];
+  float s[kGatherRows];
+#pragma unroll
+  for (int k = 0; k < kGatherRows; ++k) {
+    w[k] = make_uint4(0x80808080u, 0x80808080u, 0x80808080u, 0x80808080u);
+    s[k] = 0.f;
+    if (page[k] >= 0) {
+      const int row = (f + i0 + k * side) & ((1 << p.m.shift) - 1);
+      w[k] = *reinterpret_cast<const uint4*>(p.c.codes + code_offset(p.m, page[k], h, row) + ch);
+      s[k] = p.c.scale[scale_offset(p.m, page[k], h, row)];
+    }
   }
-  uint4* o = reinterpret_cast<uint4*>(out + r * m.D + ch);
-  o[0] = lo;
-  o[1] = hi;
+#pragma unroll
+  for (int k = 0; k < kGatherRows; ++k) {
+    const int i = i0 + k * side;
+    if (i >= p.n) continue;
+    uint4* o = reinterpret_cast<uint4*>(p.out + (((int64_t)b * p.n + i) * p.m.Hkv + h) * p.m.D + ch);
+    const uint2 a = four(w[k].x, s[k]), bb = four(w[k].y, s[k]), c = four(w[k].z, s[k]), d = four(w[k].w, s[k]);
+    o[0] = make_uint4(a.x, a.y, bb.x, bb.y);
+    o[1] = make_uint4(c.x, c.y, d.x, d.y);
+  }
 }
 
 // ------------------------------------------------------------------ attention
@@ -297,11 +353,20 @@ __device__ __forceinline__ uint2 ld_stream8(const void* p) {
   asm volatile("ld.global.nc.L1::no_allocate.v2.u32 {%0,%1}, [%2];" : "=r"(v.x), "=r"(v.y) : "l"(p));
   return v;
 }
+// A constant that stays in a register: written as an immediate, it is moved into one again for each use.
+__device__ __forceinline__ uint32_t in_register(uint32_t c) {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %1;" : "=r"(r) : "r"(c));
+  return r;
+}
+struct Consts {
+  uint32_t high, minus;  // 0x64646464 (the high bytes of fp16 1024 + u), 0xe480e480 (-1152)
+};
 // fp16 pair of two biased codes: bytes (sel) of w become 1024 + u, minus 1152
 template <int kSel>
-__device__ __forceinline__ uint32_t half2_of(uint32_t w) {
-  uint32_t x = __byte_perm(w, 0x64646464u, kSel), r;
-  asm("sub.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x64806480u));
+__device__ __forceinline__ uint32_t half2_of(uint32_t w, const Consts& k) {
+  uint32_t x = __byte_perm(w, k.high, kSel), r;
+  asm("add.rn.f16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(k.minus));
   return r;
 }
 __device__ __forceinline__ void mma_f16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -314,6 +379,11 @@ __device__ __forceinline__ uint32_t transpose8x8(uint32_t v) {
   uint32_t r;
   asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(r) : "r"(v));
   return r;
+}
+__device__ __forceinline__ float ex2(float x) {  // 2^x to 2^-22, 0 below 2^-126
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
 __device__ __forceinline__ uint32_t pack_f16(float lo, float hi) {
   __half2 h = __floats2half2_rn(lo, hi);
@@ -345,8 +415,11 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int r = lane >> 2, t = lane & 3;
   const int V = p.m.Hkv * p.hg;
+  const Consts konst{in_register(0x64646464u), in_register(0xe480e480u)};
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
 
-  // prefix of the steps (kWarps blocks) of every sequence
+  // prefix of the steps (kWarps blocks) of every sequence; the host has checked that all of them fit 31 bits
   int carry = 0;
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
     int n = 0;
@@ -370,84 +443,35 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
       carry += s_warp[w];
     }
     if (b0 + tid < p.B) s_pre[b0 + tid] = before + x - n;
+    if (b0 + tid == p.B - 1) s_pre[p.B] = before + x;
     __syncthreads();
   }
-  if (tid == 0) s_pre[p.B] = carry;
-  // sequences without a key: zero rows, written by the last CTAs (they have the least to do)
-  for (int b = gridDim.x - 1 - blockIdx.x; b < p.B; b += gridDim.x) {
-    int len, lo, first, count;
-    blocks_of(p, b, len, lo, first, count);
-    if (count == 0)
-      for (int i = tid; i < p.Hq * D / 8; i += kThreads)
-        *reinterpret_cast<uint4*>(p.out + (int64_t)b * p.o_rs + i * 8) = make_uint4(0, 0, 0, 0);
-  }
-  const int64_t total = (int64_t)carry * V;
-  const int64_t per = max((total + gridDim.x - 1) / gridDim.x, (int64_t)kMinSteps);
-  int64_t at = blockIdx.x * per;
-  const int64_t end = min(total, at + per);
-  if (at >= end) return;
-  __syncthreads();
+  const int total = carry * V;
+  const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, kMinSteps);
+  int at = blockIdx.x * per;
+  const int end = min(total, at + per);
   int b = 0;
-  {  // the last sequence that starts at or before `at` and is not empty
+  if (at < end) {  // the last sequence that starts at or before `at`
     int hi = p.B;
     while (hi - b > 1) {
       const int mid = (b + hi) >> 1;
-      if ((int64_t)s_pre[mid] * V <= at) b = mid; else hi = mid;
+      if (s_pre[mid] * V <= at) b = mid; else hi = mid;
     }
   }
   while (at < end) {
-    while (s_pre[b + 1] == s_pre[b] || (int64_t)s_pre[b + 1] * V <= at) ++b;
+    while (s_pre[b + 1] == s_pre[b] || s_pre[b + 1] * V <= at) ++b;
     const int steps = s_pre[b + 1] - s_pre[b];
-    const int64_t off = at - (int64_t)s_pre[b] * V;
-    const int v = (int)(off / steps), st0 = (int)(off % steps);
-    const int st1 = (int)min((int64_t)steps, st0 + (end - at));
-    const int hk = v / p.hg, h0 = hk * p.G + (v % p.hg) * 8;
-    const int heads = min(8, p.G - (v % p.hg) * 8);
+    const int off = at - s_pre[b] * V;
+    const int v = off / steps, st0 = off - v * steps;
+    const int st1 = min(steps, st0 + (end - at));
+    const int hk = v / p.hg, h0 = hk * p.G + (v - hk * p.hg) * 8;
+    const int heads = min(8, p.G - (v - hk * p.hg) * 8);
     int len, lo, first, count;
     blocks_of(p, b, len, lo, first, count);
     const int slot = p.slot[b];
     const int blk0 = first + st0 * kWarps + warp;              // this warp's blocks: blk0, blk0 + kWarps, ...
     const int blk1 = min(first + count, first + st1 * kWarps);
     const int n_blk = blk1 > blk0 ? (blk1 - blk0 + kWarps - 1) / kWarps : 0;
-
-    // q as the B operand: head r, dims 16 t .. of each 64
-    uint32_t qb[kKs][2];
-    float fac0, fac1;
-    {
-      const bool ok = r < heads;
-      const __nv_bfloat16* qr = p.q + (int64_t)b * p.q_rs + (int64_t)(h0 + (ok ? r : 0)) * D + t * 16;
-      float f[kKs * 4];
-      uint32_t top = 0;
-#pragma unroll
-      for (int i = 0; i < kKl; ++i)
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          float e8[8];
-          dec::unpack8(*reinterpret_cast<const uint4*>(qr + i * 64 + j * 8), e8);
-#pragma unroll
-          for (int e = 0; e < 8; ++e) {
-            f[i * 16 + j * 8 + e] = ok ? e8[e] : 0.f;
-            top = max(top, __float_as_uint(f[i * 16 + j * 8 + e]) & 0x7fffffffu);
-          }
-        }
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
-      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      int k = top == 0 || top >= 0x7f800000u ? 0 : 13 + 127 - (int)(top >> 23);  // largest |q| into [2^13, 2^14)
-      k = min(k, 100);
-      const float up = __uint_as_float((uint32_t)(127 + k) << 23), down = __uint_as_float((uint32_t)(127 - k) << 23);
-#pragma unroll
-      for (int i = 0; i < kKs; ++i) {
-        qb[i][0] = pack_f16(f[4 * i] * up, f[4 * i + 1] * up);
-        qb[i][1] = pack_f16(f[4 * i + 2] * up, f[4 * i + 3] * up);
-      }
-      const float fac = (CAP ? p.cap_in : p.scale_log2) * down;
-      fac0 = __shfl_sync(0xffffffffu, fac, 8 * t);  // heads 2 t and 2 t + 1
-      fac1 = __shfl_sync(0xffffffffu, fac, 8 * t + 4);
-    }
-    float o[kKs][4];
-#pragma unroll
-    for (int i = 0; i < kKs; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
-    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
 
     uint4 kr[2 * kKl];   // rows r and r + 8
     uint4 vr[4];         // rows 2 t, 2 t + 1, 2 t + 8, 2 t + 9 (D = 64: the low half of each)
@@ -477,33 +501,84 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
         }
       }
     };
-    for (int i0 = 0; i0 < n_blk; i0 += 32) {
-      const int nb = min(32, n_blk - i0);
-      // records of this warp's next 32 blocks: page, key scale, log2 and inverse of the value scale
-      __syncwarp();
-      if (lane < nb) {
-        const int pos = (blk0 + (i0 + lane) * kWarps) << 4;
-        const int page = page_of(p.m, slot, pos, p.status);
-        float ks = 0.f, lv = -INFINITY, inv = 0.f;  // an unusable page: weights of zero
-        if (page >= 0) {
-          const int64_t so = scale_offset(p.m, page, hk, pos & ((1 << p.m.shift) - 1));
-          ks = p.k.scale[so];
-          float vs = p.v.scale[so];
-          vs = vs < 6.2e-33f ? 6.2e-33f : vs;  // (a NaN stays)
-          lv = log2f(vs);
-          inv = 1.f / vs;
-        }
-        s_rec[lane] = make_int4(max(page, 0), __float_as_int(ks), __float_as_int(lv), __float_as_int(inv));
-      }
-      __syncwarp();
-      int64_t base = block_base(s_rec[0].x, blk0 + i0 * kWarps);
+    // Records of this warp's next 32 blocks: page, key scale, log2 and inverse of the value scale. The first block's
+    // codes are asked for as soon as its page is known, beside the scales.
+    auto fill = [&](int i0) {
+      int page = -1;
+      const int pos = (blk0 + (i0 + lane) * kWarps) << 4;
+      if (i0 + lane < n_blk) page = page_of(p.m, slot, pos, p.status);
+      const int64_t base = block_base(max(__shfl_sync(0xffffffffu, page, 0), 0), blk0 + i0 * kWarps);
       load_k(base);
       load_v(base);
+      float ks = 0.f, vs = 0.f;
+      if (page >= 0) {
+        const int64_t so = scale_offset(p.m, page, hk, pos & ((1 << p.m.shift) - 1));
+        ks = p.k.scale[so];
+        vs = p.v.scale[so];
+      }
+      vs = vs < 6.2e-33f ? 6.2e-33f : vs;  // (a NaN stays)
+      __syncwarp();
+      // an unusable page has weights of zero
+      s_rec[lane] = make_int4(max(page, 0), __float_as_int(ks), __float_as_int(page >= 0 ? log2f(vs) : -INFINITY),
+                              __float_as_int(page >= 0 ? 1.f / vs : 0.f));
+      __syncwarp();
+    };
+    uint4 qraw[kKl][2];  // head r, dims 16 t .. of each 64
+    {
+      const __nv_bfloat16* qr = p.q + (int64_t)b * p.q_rs + (int64_t)(h0 + (r < heads ? r : 0)) * D + t * 16;
+#pragma unroll
+      for (int i = 0; i < kKl; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) qraw[i][j] = *reinterpret_cast<const uint4*>(qr + i * 64 + j * 8);
+    }
+    if (n_blk > 0) fill(0);
+
+    // q as the B operand
+    uint32_t qb[kKs][2];
+    float fac0, fac1;
+    {
+      const bool ok = r < heads;
+      float f[kKs * 4];
+      uint32_t top = 0;
+#pragma unroll
+      for (int i = 0; i < kKl; ++i)
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          float e8[8];
+          dec::unpack8(qraw[i][j], e8);
+#pragma unroll
+          for (int e = 0; e < 8; ++e) {
+            f[i * 16 + j * 8 + e] = ok ? e8[e] : 0.f;
+            top = max(top, __float_as_uint(f[i * 16 + j * 8 + e]) & 0x7fffffffu);
+          }
+        }
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = max(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      int k = top == 0 || top >= 0x7f800000u ? 0 : 13 + 127 - (int)(top >> 23);  // largest |q| into [2^13, 2^14)
+      k = min(k, 100);
+      const float up = __uint_as_float((uint32_t)(127 + k) << 23), down = __uint_as_float((uint32_t)(127 - k) << 23);
+#pragma unroll
+      for (int i = 0; i < kKs; ++i) {
+        qb[i][0] = pack_f16(f[4 * i] * up, f[4 * i + 1] * up);
+        qb[i][1] = pack_f16(f[4 * i + 2] * up, f[4 * i + 3] * up);
+      }
+      const float fac = (CAP ? p.cap_in : p.scale_log2) * down;
+      fac0 = __shfl_sync(0xffffffffu, fac, 8 * t);  // heads 2 t and 2 t + 1
+      fac1 = __shfl_sync(0xffffffffu, fac, 8 * t + 4);
+    }
+    float o[kKs][4];
+#pragma unroll
+    for (int i = 0; i < kKs; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
+    float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+
+    for (int i0 = 0; i0 < n_blk; i0 += 32) {
+      const int nb = min(32, n_blk - i0);
+      if (i0 > 0) fill(i0);
       for (int i = 0; i < nb; ++i) {
         const int4 rec = s_rec[i];
         const int pos = (blk0 + (i0 + i) * kWarps) << 4;
         const int nx = min(i + 1, nb - 1);
-        base = block_base(s_rec[nx].x, blk0 + (i0 + nx) * kWarps);
+        const int64_t base = block_base(s_rec[nx].x, blk0 + (i0 + nx) * kWarps);
         float c[4] = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
         for (int j = 0; j < kKl; ++j) {
@@ -511,8 +586,8 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
           const uint32_t wh[4] = {kr[kKl + j].x, kr[kKl + j].y, kr[kKl + j].z, kr[kKl + j].w};
 #pragma unroll
           for (int e = 0; e < 4; ++e) {
-            const uint32_t a[4] = {half2_of<0x4140>(wl[e]), half2_of<0x4140>(wh[e]), half2_of<0x4342>(wl[e]),
-                                   half2_of<0x4342>(wh[e])};
+            const uint32_t a[4] = {half2_of<0x4140>(wl[e], konst), half2_of<0x4140>(wh[e], konst), half2_of<0x4342>(wl[e], konst),
+                                   half2_of<0x4342>(wh[e], konst)};
             mma_f16(c, a, qb[4 * j + e][0], qb[4 * j + e][1]);
           }
         }
@@ -542,7 +617,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
           }
           n0 = fmaxf(n0, m0);
           n1 = fmaxf(n1, m1);
-          const float a0 = n0 == -INFINITY ? 1.f : exp2f(m0 - n0), a1 = n1 == -INFINITY ? 1.f : exp2f(m1 - n1);
+          const float a0 = n0 == -INFINITY ? 1.f : ex2(m0 - n0), a1 = n1 == -INFINITY ? 1.f : ex2(m1 - n1);
           m0 = n0;
           m1 = n1;
           l0 *= a0;
@@ -557,7 +632,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
         }
         const float d0 = lv + kWeightBits - (m0 == -INFINITY ? 0.f : m0);
         const float d1 = lv + kWeightBits - (m1 == -INFINITY ? 0.f : m1);
-        const float w0 = exp2f(x[0] + d0), w1 = exp2f(x[1] + d1), w2 = exp2f(x[2] + d0), w3 = exp2f(x[3] + d1);
+        const float w0 = ex2(x[0] + d0), w1 = ex2(x[1] + d1), w2 = ex2(x[2] + d0), w3 = ex2(x[3] + d1);
         l0 = fmaf(w0 + w2, inv, l0);
         l1 = fmaf(w1 + w3, inv, l1);
         const uint32_t pb0 = transpose8x8(pack_f16(w0, w1)), pb1 = transpose8x8(pack_f16(w2, w3));
@@ -570,7 +645,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
 #pragma unroll
           for (int e = 0; e < 2; ++e) {  // dims (D / 8) r + 4 j + 2 e (rows r) and the next (rows r + 8)
             const uint32_t ab = __byte_perm(wa, wb, e ? 0x7362 : 0x5140), cd = __byte_perm(wc, wd, e ? 0x7362 : 0x5140);
-            const uint32_t a[4] = {half2_of<0x4140>(ab), half2_of<0x4342>(ab), half2_of<0x4140>(cd), half2_of<0x4342>(cd)};
+            const uint32_t a[4] = {half2_of<0x4140>(ab, konst), half2_of<0x4342>(ab, konst), half2_of<0x4140>(cd, konst), half2_of<0x4342>(cd, konst)};
             mma_f16(o[2 * j + e], a, pb0, pb1);
           }
         }
@@ -597,9 +672,9 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
     }
     __syncthreads();
     const bool whole = st0 == 0 && st1 == steps;
-    const int64_t seg0 = (int64_t)s_pre[b] * V + (int64_t)v * steps;  // the segment's first step
-    const int64_t cta0 = seg0 / per;
-    float* part = p.parts + ((int64_t)blockIdx.x * 2 + (cta0 == blockIdx.x ? 1 : 0)) * kPartFloats;
+    const int seg0 = s_pre[b] * V + v * steps;  // the segment's first step
+    const int cta0 = seg0 / per;
+    float* part = p.parts + ((int64_t)blockIdx.x * 2 + (cta0 == (int)blockIdx.x ? 1 : 0)) * kPartFloats;
     constexpr int kPer = 8 * D / kThreads;  // consecutive dims of one head for each thread
     {
       const int g = tid * kPer / D, d = tid * kPer % D;
@@ -612,7 +687,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
         const float mw = s_m[w * 8 + g];
-        const float f = mw == -INFINITY ? (s_l[w * 8 + g] == 0.f ? 0.f : 1.f) : exp2f(mw - mm);  // l is 0 or NaN
+        const float f = mw == -INFINITY ? (s_l[w * 8 + g] == 0.f ? 0.f : 1.f) : ex2(mw - mm);  // l is 0 or NaN
         ll += f * s_l[w * 8 + g];
 #pragma unroll
         for (int e = 0; e < kPer; ++e) acc[e] += f * s_o[(w * 8 + g) * D + d + e];
@@ -635,56 +710,60 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
       }
     }
     if (!whole) {
-      const int64_t cta1 = (seg0 + steps - 1) / per;
-      const int np = (int)(cta1 - cta0) + 1;
+      const int np = (seg0 + steps - 1) / per - cta0 + 1;
       __threadfence();
       __syncthreads();
       if (tid == 0) s_flag = atomicAdd(p.counters + b * V + v, 1) == np - 1;
       __syncthreads();
       if (s_flag) {
         __threadfence();
-        auto part_of = [&](int i) { return p.parts + ((cta0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats; };
-        {  // warp g: the parts' weights for head g, 2^(M_i - M) / l
-          const int g = warp;
-          float* wgt = s_o + g * kMaxCtas;
-          float mm = -INFINITY;
-          for (int i = lane; i < np; i += 32) mm = fmaxf(mm, __ldcg(part_of(i) + 8 * D + g));
-          mm = warp_max(mm);
-          float ll = 0.f;
-          for (int i = lane; i < np; i += 32) {
-            const float mi = __ldcg(part_of(i) + 8 * D + g), li = __ldcg(part_of(i) + 8 * D + 8 + g);
-            const float f = mi == -INFINITY ? (li == 0.f ? 0.f : 1.f) : exp2f(mi - mm);
-            wgt[i] = f;
-            ll += f * li;
+        auto part_of = [&](int i) { return p.parts + ((int64_t)(cta0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats; };
+        constexpr int kBatch = 16;  // parts in flight
+        const int g = tid * kPer / D, d = tid * kPer % D;
+        float pv[kBatch][kPer];
+        auto load_parts = [&](int i0) {
+#pragma unroll
+          for (int i = 0; i < kBatch; ++i) {
+            const float* src = part_of(min(i0 + i, np - 1)) + g * D + d;
+            if constexpr (kPer == 4) {
+              const float4 q4 = __ldcg(reinterpret_cast<const float4*>(src));
+              pv[i][0] = q4.x, pv[i][1] = q4.y, pv[i][2] = q4.z, pv[i][3] = q4.w;
+            } else {
+              const float2 q2 = __ldcg(reinterpret_cast<const float2*>(src));
+              pv[i][0] = q2.x, pv[i][1] = q2.y;
+            }
           }
-          ll = warp_sum(ll);
-          __syncwarp();
-          for (int i = lane; i < np; i += 32) wgt[i] *= ll == 0.f ? 0.f : 1.f / ll;
+        };
+        load_parts(0);
+        {  // warp h: the parts' weights for head h, 2^(M_i - M) / l
+          float* wgt = s_o + warp * kMaxCtas;
+          float mm = -INFINITY, ll = 0.f;
+          for (int i = lane; i < np; i += 32) {
+            const float mi = __ldcg(part_of(i) + 8 * D + warp), li = __ldcg(part_of(i) + 8 * D + 8 + warp);
+            const float mn = fmaxf(mm, mi);
+            const float f = mi == -INFINITY ? (li == 0.f ? 0.f : 1.f) : 1.f;
+            ll = ll * (mm == -INFINITY ? 1.f : ex2(mm - mn)) + li * f * (mi == -INFINITY ? 1.f : ex2(mi - mn));
+            mm = mn;
+            wgt[i] = f == 0.f ? -INFINITY : mi;
+          }
+          const float ml = mm;
+          mm = warp_max(mm);
+          ll = warp_sum(ll * (ml == -INFINITY ? 1.f : ex2(ml - mm)));
+          const float inv = ll == 0.f ? 0.f : 1.f / ll;
+          for (int i = lane; i < np; i += 32) wgt[i] = (wgt[i] == -INFINITY ? 0.f : ex2(wgt[i] - mm)) * inv;
         }
         __syncthreads();
-        const int g = tid * kPer / D, d = tid * kPer % D;
         const float* wgt = s_o + g * kMaxCtas;
         float acc[kPer];
 #pragma unroll
         for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-        for (int i0 = 0; i0 < np; i0 += 8) {
-          float x[8][kPer];
+        for (int i0 = 0; i0 < np; i0 += kBatch) {
+          if (i0 > 0) load_parts(i0);
 #pragma unroll
-          for (int i = 0; i < 8; ++i) {
-            const float* src = part_of(min(i0 + i, np - 1)) + g * D + d;
-            if constexpr (kPer == 4) {
-              const float4 q4 = __ldcg(reinterpret_cast<const float4*>(src));
-              x[i][0] = q4.x, x[i][1] = q4.y, x[i][2] = q4.z, x[i][3] = q4.w;
-            } else {
-              const float2 q2 = __ldcg(reinterpret_cast<const float2*>(src));
-              x[i][0] = q2.x, x[i][1] = q2.y;
-            }
-          }
-#pragma unroll
-          for (int i = 0; i < 8; ++i)
+          for (int i = 0; i < kBatch; ++i)
             if (i0 + i < np) {
 #pragma unroll
-              for (int e = 0; e < kPer; ++e) acc[e] += wgt[i0 + i] * x[i][e];
+              for (int e = 0; e < kPer; ++e) acc[e] += wgt[i0 + i] * pv[i][e];
             }
         }
         if (g < heads) {
@@ -698,9 +777,31 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
     __syncthreads();  // the sums are free again
     at += st1 - st0;
   }
+  // sequences without a key: zero rows
+  for (b = blockIdx.x; b < p.B; b += gridDim.x) {
+    if (s_pre[b + 1] != s_pre[b]) continue;
+    for (int i = tid; i < p.Hq * D / 8; i += kThreads)
+      *reinterpret_cast<uint4*>(p.out + (int64_t)b * p.o_rs + i * 8) = make_uint4(0, 0, 0, 0);
+  }
 }
 
 // ------------------------------------------------------------------ host
+// Launch that may begin while the kernel before it in the stream drains; every kernel here waits for that one to
+// complete (griddepcontrol.wait) before it touches memory, and only then lets its own successor begin.
+template <typename P>
+static void launch_pdl(void (*kernel)(P), dim3 grid, dim3 block, int smem, cudaStream_t st, const P& p) {
+  cudaLaunchConfig_t cfg{};
+  cfg.gridDim = grid;
+  cfg.blockDim = block;
+  cfg.dynamicSmemBytes = smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at{};
+  at.id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at.val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = &at;
+  cfg.numAttrs = 1;
+  AETHER_CUDA_CHECK(cudaLaunchKernelEx(&cfg, kernel, p));
+}
 static void check_pool(const at::Tensor& codes, const at::Tensor& scale, const at::Tensor& table, const char* what) {
   TORCH_CHECK(codes.is_cuda() && codes.scalar_type() == at::kByte && codes.dim() == 4 && codes.is_contiguous(), what,
               ": codes are contiguous CUDA uint8 [pages, Hkv, page, D]");
@@ -795,48 +896,63 @@ void rope_kv8_append(at::Tensor qkv, at::Tensor pos, at::Tensor slot, std::optio
   p.max_pos = (int)std::min<int64_t>(cos_t.size(0), (int64_t(1) << 31) - 1);
   p.T = T;
   p.status = device_status_word();
-  const dim3 grid((unsigned)units, (unsigned)((Hq + 2 * Hkv + 3) / 4));
+  // a warp for each head while there are few blocks; a CTA that walks over the heads once they fill the GPU
+  const int64_t all = (Hq + 2 * Hkv + kAppendWarps - 1) / kAppendWarps;
+  const int64_t spread = std::max<int64_t>(1, std::min<int64_t>(all, 8 * num_sms(current_device()) / units));
+  const dim3 grid((unsigned)units, (unsigned)spread);
   auto st = at::cuda::getCurrentCUDAStream();
-  if (D == 128)
-    append_kernel<128><<<grid, 128, 0, st>>>(p);
-  else
-    append_kernel<64><<<grid, 128, 0, st>>>(p);
-  AETHER_CUDA_CHECK(cudaGetLastError());
+  launch_pdl(D == 128 ? append_kernel<128> : append_kernel<64>, grid, dim3(kAppendWarps * 32), 0, st, p);
 }
 
-void gather_kv8(at::Tensor codes, at::Tensor scale, at::Tensor page_table, at::Tensor slot,
-                std::optional<at::Tensor> first, int64_t first0, at::Tensor out) {
+at::Tensor gather_kv8(at::Tensor codes, at::Tensor scale, at::Tensor page_table, at::Tensor slot,
+                      std::optional<at::Tensor> first, int64_t first0, int64_t n, std::optional<at::Tensor> into) {
   using namespace kv8;
   check_pool(codes, scale, page_table, "gather_kv8");
+  TORCH_CHECK(slot.dim() == 1 && n >= 0, "gather_kv8: slot [B] and a length");
+  const int64_t B = slot.size(0);
+  const at::Tensor out = into && into->defined()
+                             ? *into
+                             : at::empty({B, n, codes.size(1), codes.size(3)}, codes.options().dtype(at::kBFloat16));
   TORCH_CHECK(out.device() == codes.device() && out.scalar_type() == at::kBFloat16 && out.dim() == 4 &&
-                  out.is_contiguous() && out.size(2) == codes.size(1) && out.size(3) == codes.size(3) &&
+                  out.is_contiguous() && out.size(0) == B && out.size(1) == n && out.size(2) == codes.size(1) && out.size(3) == codes.size(3) &&
                   reinterpret_cast<uintptr_t>(out.data_ptr()) % 16 == 0,
               "gather_kv8: out is contiguous bf16 [B, n, Hkv, D]");
-  const int64_t B = out.size(0), n = out.size(1);
   check_ints(slot, codes, B, "gather_kv8: slot [B]");
   const bool each = first && first->defined();
   if (each) check_ints(*first, codes, B, "gather_kv8: first [B]");
   TORCH_CHECK(n < (int64_t(1) << 31) && first0 >= 0 && first0 + n < (int64_t(1) << 31), "gather_kv8: positions");
-  const int64_t total = out.numel() / 16;
-  if (total == 0) return;
+  TORCH_CHECK(B <= 65535, "gather_kv8: at most 65535 sequences");
+  if (out.numel() == 0) return out;
   c10::cuda::CUDAGuard g(codes.device());
-  TORCH_CHECK((total + 255) / 256 < (int64_t(1) << 31), "gather_kv8: output too large");
-  gather_kernel<<<(unsigned)((total + 255) / 256), 256, 0, at::cuda::getCurrentCUDAStream()>>>(
-      pool_of(codes, scale), make_map(codes, page_table), slot.data_ptr<int>(), each ? first->data_ptr<int>() : nullptr,
-      (int)first0, n, total, reinterpret_cast<__nv_bfloat16*>(out.data_ptr()), device_status_word());
-  AETHER_CUDA_CHECK(cudaGetLastError());
+  GatherParams p{};
+  p.c = pool_of(codes, scale);
+  p.m = make_map(codes, page_table);
+  p.slot = slot.data_ptr<int>();
+  p.first = each ? first->data_ptr<int>() : nullptr;
+  p.first0 = (int)first0;
+  p.n = (int)n;
+  p.heads = std::min(p.m.Hkv, kGatherThreads / (p.m.D / 16));
+  p.out = reinterpret_cast<__nv_bfloat16*>(out.data_ptr());
+  p.status = device_status_word();
+  const int rows = kGatherThreads / (p.m.D / 16 * p.heads) * kGatherRows;
+  launch_pdl(gather_kernel, dim3((unsigned)((n + rows - 1) / rows), (unsigned)B, (unsigned)((p.m.Hkv + p.heads - 1) / p.heads)),
+             dim3(kGatherThreads), 0, at::cuda::getCurrentCUDAStream(), p);
+  return out;
 }
 
-void kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor vc, at::Tensor vs,
-                          at::Tensor page_table, at::Tensor slot, at::Tensor seqlen, at::Tensor out, int64_t Hq,
-                          double scale, at::Tensor workspace, int64_t window, double softcap) {
+at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor vc, at::Tensor vs,
+                                at::Tensor page_table, at::Tensor slot, at::Tensor seqlen,
+                                std::optional<at::Tensor> into, int64_t Hq, double scale, at::Tensor workspace,
+                                int64_t window, double softcap) {
   using namespace kv8;
   check_pool(kc, ks, page_table, "kv8_decode_attention");
   check_pool(vc, vs, page_table, "kv8_decode_attention");
   check_same(kc, vc, "kv8_decode_attention");
+  TORCH_CHECK(q.dim() == 2, "kv8_decode_attention: q is [B, >= Hq D]");
   const int64_t Hkv = kc.size(1), D = kc.size(3), B = q.size(0);
   TORCH_CHECK(Hq >= Hkv && Hq % Hkv == 0, "kv8_decode_attention: query heads are a multiple of the KV heads");
-  for (const at::Tensor* t : {&q, &out})
+  const at::Tensor out = into && into->defined() ? *into : at::empty({B, Hq * D}, q.options());
+  for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&q, &out})
     TORCH_CHECK(t->device() == kc.device() && t->dim() == 2 && t->scalar_type() == at::kBFloat16 && t->size(0) == B &&
                     t->size(1) >= Hq * D && t->stride(1) == 1 && t->stride(0) % 8 == 0 &&
                     reinterpret_cast<uintptr_t>(t->data_ptr()) % 16 == 0,
@@ -850,7 +966,7 @@ void kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor
   TORCH_CHECK(workspace.device() == kc.device() && workspace.scalar_type() == at::kByte && workspace.is_contiguous() &&
                   workspace.numel() >= kWorkspaceBytes && reinterpret_cast<uintptr_t>(workspace.data_ptr()) % 16 == 0,
               "kv8_decode_attention: workspace from kv8_workspace on the cache's device");
-  if (B == 0) return;
+  if (B == 0) return out;
   c10::cuda::CUDAGuard g(kc.device());
   AttnParams p{};
   p.q = reinterpret_cast<const __nv_bfloat16*>(q.data_ptr());
@@ -878,6 +994,7 @@ void kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor
   int64_t keys = (int64_t)p.m.cols << p.m.shift;
   if (window > 0) keys = std::min<int64_t>(keys, window + kBlock);
   const int64_t most = B * Hkv * hg * std::max<int64_t>(1, (keys + kWarps * kBlock - 1) / (kWarps * kBlock));
+  TORCH_CHECK(most < (int64_t(1) << 30), "kv8_decode_attention: the page table's positions times sequences and heads");
   const int grid = (int)std::min<int64_t>(std::min(2 * num_sms(current_device()), kMaxCtas), most);
   const int smem = kSmemFixed + ((int)B + 1) * 4;
   auto st = at::cuda::getCurrentCUDAStream();
@@ -888,8 +1005,7 @@ void kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor
                                              kSmemFixed + (kMaxSeqs + 1) * 4));
       set[dev] = true;
     }
-    kernel<<<grid, kThreads, smem, st>>>(p);
-    AETHER_CUDA_CHECK(cudaGetLastError());
+    launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, st, p);
   };
   static bool set[4][64] = {};
   if (D == 128 && softcap > 0)
@@ -900,6 +1016,7 @@ void kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor
     launch(attn_kernel<64, true>, set[2]);
   else
     launch(attn_kernel<64, false>, set[3]);
+  return out;
 }
 
 }  // namespace aether

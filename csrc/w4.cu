@@ -42,39 +42,48 @@ struct LinearParams {
   int64_t rs;
   __nv_bfloat16* y;
   int64_t ys;
-  int M, n_out, swiglu, x_aligned, stage;  // stage: column tiles of x in shared memory at a time
+  int M, n_out, swiglu;
+  int outs, tiles, S, per;  // outputs of a CTA and how many such; parts of the columns and their column tiles
+  int* status;
 };
 
-// A CTA of eight warps owns 128 rows (SwiGLU: 64 gate rows and the 64 up rows
-// they meet) and, in a cluster of S, the S-th part of the columns. A warp
-// streams 16 rows: one column tile is two 16-byte loads a thread, kept kAhead
-// tiles ahead in registers, and its nibbles become the A operand of m16n8k16
-// steps without a shuffle -- (w >> 4 i) & 0xf | 0x4300 is bf16 128 + code, minus
-// 136 the exact weight code. The token rows (B operand, eight to a step) sit in
-// shared memory, whose rows are 32 bytes apart modulo 128, so that a quad's
-// 8-byte reads of four rows meet no bank twice. A group's sum of exact
-// products stays in fp32 and is scaled once. The CTAs of a cluster add their
-// sums over distributed shared memory, each its share of the outputs in the
-// order of the columns, so no workspace is needed and the result is the same
-// on every run.
-constexpr int kWarps = 8;
-constexpr int kThreads = kWarps * 32;
-constexpr int kRows = kWarps * 16;
-constexpr int kSumLd = kRows + 4;  // floats of one token's sums
-constexpr int kStageBytes = 72 * 1024;
+// A CTA's eight multiplying warps own 128 / KH rows, a tile of 16 each (SwiGLU:
+// gate tiles and the up tiles they meet), and, in a cluster of S, the S-th part
+// of the columns, in KH parts that warps take side by side. Each streams its
+// codes and scales through its own ring in shared memory, six of eight column
+// tiles ahead (16-byte asynchronous copies: 16 warps keep about 100 KB in flight
+// on an SM, and half of that reads at two thirds of the rate). A ninth warp
+// brings the token rows, 4 / KH column tiles at a time, into one of two buffers
+// that the eight share (bulk copies of its 512-byte rows took 65 ns each). A lane's 16 bytes of a weight row become
+// the A operand of m16n8k16 steps without a shuffle -- (w >> 4 i) & 0xf | 0x4300
+// is bf16 128 + code, minus 136 the exact weight code. Token rows (B operand,
+// eight to a step) lie 32 bytes apart modulo 128, so that a quad's 8-byte reads
+// of four rows meet no bank twice. A group's sum of exact products stays in fp32
+// and is scaled once. The CTAs of a cluster add their sums over distributed
+// shared memory, each its share of the outputs in the order of the columns, so
+// no workspace is needed and the result is the same on every run.
+// Bound by the issue of the unpacking (11 instructions for eight weights, about
+// 125 for a warp's column tile) beside the weights' bytes.
+constexpr int kWarps = 8;                   // that multiply
+constexpr int kThreads = kWarps * 32 + 32;
+constexpr int kPair = 2;                    // column tiles of a ring stage
+constexpr int kRing = 4;                    // stages of a warp's ring
 
-__device__ __forceinline__ uint4 ld_stream16(const void* p) {
-  uint4 v;
-  asm volatile("ld.global.nc.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
-               : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "l"(p));
-  return v;
+// A constant that stays in a register: written as an immediate, it is moved into one again for each use.
+__device__ __forceinline__ uint32_t in_register(uint32_t c) {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %1;" : "=r"(r) : "r"(c));
+  return r;
 }
+struct Consts {
+  uint32_t mask, bias, minus;  // 0x000f000f, 0x43004300 (128), 0xc308c308 (-136)
+};
 // bf16 pair of two weight codes (nibbles i and i + 4 of w), exact
 template <int i>
-__device__ __forceinline__ uint32_t codes2(uint32_t w) {
+__device__ __forceinline__ uint32_t codes2(uint32_t w, const Consts& k) {
   uint32_t x, r;
-  asm("lop3.b32 %0, %1, 0x000f000f, 0x43004300, 0xea;" : "=r"(x) : "r"(w >> (4 * i)));  // (a & b) | c
-  asm("sub.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(0x43084308u));
+  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w >> (4 * i)), "r"(k.mask), "r"(k.bias));  // (a & b) | c
+  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(k.minus));
   return r;
 }
 __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
@@ -83,205 +92,310 @@ __device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], 
       : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
       : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ld_cluster(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
+               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ uint32_t cluster_size() {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %%cluster_nctaid.x;" : "=r"(r));
-  return r;
+__device__ __forceinline__ uint4 lds128(uint32_t addr) {
+  uint4 v;
+  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
+  uint32_t v;
+  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
+}
+__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool in) {  // zeros where not `in`
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 
-// MT: tiles of eight token rows; GS: k16 steps of a scale group (2, 4 or 8)
-template <int MT, int GS>
+// MT: tiles of eight token rows; GS: k16 steps of a scale group (2, 4 or 8); KH: parts of the columns side by side
+template <int MT, int GS, int KH>
 __global__ void __launch_bounds__(kThreads, MT <= 2 ? 2 : 1) linear_kernel(LinearParams p) {
-  constexpr int kAhead = MT <= 2 ? 4 : 2;
-  extern __shared__ __align__(16) uint8_t smem[];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
-  const int S = (int)cluster_size(), rank = (int)cluster_ctarank();
-  const int tile = blockIdx.x / S;
-  const int outs = p.swiglu ? kRows / 2 : kRows;  // outputs of this CTA
-  const int n0 = tile * outs;
-  const int per = (p.w.kt + S - 1) / S;
-  const int kt0 = rank * per, n_kt = max(0, min(p.w.kt, kt0 + per) - kt0);
-
-  // this lane's two weight rows (past the last row: the last row again, its sums are dropped)
-  const int warp_row = p.swiglu ? (warp < kWarps / 2 ? n0 + warp * 16 : p.n_out + n0 + (warp - kWarps / 2) * 16) : n0 + warp * 16;
-  const int ra = min(warp_row + r, p.w.N - 1), rb = min(warp_row + r + 8, p.w.N - 1);
-  auto row_q = [&](int n) {
-    return p.w.q + ((((int64_t)(n >> 4) * p.w.kt + kt0) * 2 + ((n >> 3) & 1)) * 32 + (n & 7) * 4 + t) * 4;
-  };
   constexpr int kGroups = 8 / GS;  // of a column tile
-  auto row_s = [&](int n) {
-    return p.w.s + (((int64_t)(n >> 4) * p.w.groups + (int64_t)kt0 * kGroups) * 8 + (n & 7)) * 2 + ((n >> 3) & 1);
-  };
-  const uint32_t *qa = row_q(ra), *qb = row_q(rb);
-  const __half *sa = row_s(ra), *sb = row_s(rb);
-
-  uint4 ba[kAhead], bb[kAhead];
+  constexpr int kRowTiles = kWarps / KH;
+  constexpr int kTileBytes = 1024 + kGroups * 32;
+  constexpr int kXTiles = 4 / KH;                 // column tiles of a token buffer
+  constexpr int kRowBytes = kXTiles * 256 + 32;   // a token row of it
+  extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ __align__(8) uint64_t s_full[2], s_empty[2];
+  __shared__ int s_abort;
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
+  if (tid == 0) {
+    s_abort = 0;
 #pragma unroll
-  for (int u = 0; u < kAhead; ++u)
-    if (u < n_kt) {
-      ba[u] = ld_stream16(qa + u * 256);
-      bb[u] = ld_stream16(qb + u * 256);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(s_full + i, 32);
+      mbar_init(s_empty + i, kWarps);
     }
+    fence_mbar_init();
+  }
+  const int S = p.S, rank = S > 1 ? (int)cluster_ctarank() : 0;
+  const int tile = S > 1 ? blockIdx.x / S : blockIdx.x;
+  const int n0 = tile * p.outs;                           // first output of this CTA
+  const int up = p.swiglu ? (p.n_out + n0) & 15 : 0;      // SwiGLU: where the first up row sits in its tile
+  const int c0 = rank * p.per, n_cta = max(0, min(p.w.kt, c0 + p.per) - c0);  // this CTA's column tiles
+  const int mid = KH == 1 ? n_cta : (n_cta + 1) / 2;      // of which the first part takes so many
+  const uint32_t x_at = kWarps * kRing * kPair * kTileBytes, x_bytes = KH * p.M * kRowBytes;
+  auto give_up = [&]() {
+    s_abort = 1;
+    atomicExch(p.status, kStatusTimeoutProducer);
+  };
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  __syncthreads();
   float acc[MT][4];
 #pragma unroll
   for (int m = 0; m < MT; ++m) acc[m][0] = acc[m][1] = acc[m][2] = acc[m][3] = 0.f;
-
-  // column tiles staged at a time; one row of them is ld bytes
-  const int stage = min(per, p.stage);
-  const uint32_t ld = (uint32_t)stage * 256 + 32;
-  const uint32_t xb = smem_u32(smem) + t * 8;
-  uint32_t xrow[MT];
+  if (warp == kWarps) {
+    int buf = 0, parity = 1;  // a barrier that nothing has passed lets parity 1 through
+    for (int i = 0; i < mid; i += kXTiles) {
+      if (!mbar_wait(s_empty + buf, parity, &s_abort)) give_up();
 #pragma unroll
-  for (int m = 0; m < MT; ++m) xrow[m] = xb + (uint32_t)min(m * 8 + r, p.M - 1) * ld;
-
-  int staged = 0;  // tiles before the ones in shared memory
-  for (int i0 = 0; i0 < n_kt; i0 += kAhead) {
+      for (int h = 0; h < KH; ++h) {
+        const int n = min(kXTiles, (h == 0 ? mid : n_cta - mid) - i);
+        const int k0 = (c0 + h * mid + i) * 128;
+        const uint32_t dst = smem_u32(smem) + x_at + buf * x_bytes + h * p.M * kRowBytes + lane * 16;
+        for (int m = 0; m < p.M; ++m)
 #pragma unroll
-    for (int u = 0; u < kAhead; ++u) {
-      const int i = i0 + u;
-      if (i < n_kt) {
-        if (i % stage == 0) {
-          if (i > 0) __syncthreads();
-          staged = i;
-          const int cols = min(stage, n_kt - i) * 128, k0 = (kt0 + i) * 128;
-          const int units = cols / 8;
-          for (int e = tid; e < p.M * units; e += kThreads) {
-            const int m = e / units, c = e % units * 8;
-            uint4 v = make_uint4(0, 0, 0, 0);
-            if (k0 + c < p.w.K) {
-              const __nv_bfloat16* src = p.x + m * p.xs + k0 + c;
-              if (p.x_aligned) {
-                v = __ldg(reinterpret_cast<const uint4*>(src));
-              } else {
-                const uint16_t* h = reinterpret_cast<const uint16_t*>(src);
-                v.x = h[0] | (uint32_t)h[1] << 16;
-                v.y = h[2] | (uint32_t)h[3] << 16;
-                v.z = h[4] | (uint32_t)h[5] << 16;
-                v.w = h[6] | (uint32_t)h[7] << 16;
-              }
-            }
-            *reinterpret_cast<uint4*>(smem + (uint32_t)m * ld + c * 2) = v;
+          for (int c = 0; c < kXTiles / 2; ++c) {  // 256 columns a step, zeros past K
+            const int k = k0 + c * 256 + lane * 8;
+            if (c * 2 + (lane >> 4) < n)
+              cp_async16_zfill(dst + m * kRowBytes + c * 512, p.x + m * p.xs + (k < p.w.K ? k : 0), k < p.w.K);
           }
-          __syncthreads();
+      }
+      asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(s_full + buf)) : "memory");
+      if (++buf == 2) buf = 0, parity ^= 1;
+    }
+  } else {
+    const Consts k{in_register(0x000f000fu), in_register(0x43004300u), in_register(0xc308c308u)};
+    const int kh = warp / kRowTiles, rt = warp % kRowTiles;
+    const int kt0 = c0 + kh * mid, n_kt = kh == 0 ? mid : n_cta - mid;
+    int wt = (n0 >> 4) + rt;  // packed row tile (past the last: the last, its sums are dropped)
+    if (p.swiglu && rt >= kRowTiles / 2) wt = ((p.n_out + n0) >> 4) + rt - kRowTiles / 2;
+    wt = min(wt, (p.w.N + 15) / 16 - 1);
+    const uint8_t* q = reinterpret_cast<const uint8_t*>(p.w.q) + ((int64_t)wt * p.w.kt + kt0) * 1024 + lane * 16;
+    const uint8_t* sc = reinterpret_cast<const uint8_t*>(p.w.s) + ((int64_t)wt * p.w.groups + (int64_t)kt0 * kGroups) * 32 + lane * 16;
+    const uint32_t ring = smem_u32(smem) + warp * (kRing * kPair * kTileBytes);
+    int fetched = 0;
+    uint32_t into = ring;
+    auto fetch = [&]() {  // the next stage: codes of its column tiles, then their scales
+      if (fetched < n_kt) {
+        cp_async16(into + lane * 16, q);
+        cp_async16(into + lane * 16 + 512, q + 512);
+        const bool two = fetched + 1 < n_kt;
+        if (two) {
+          cp_async16(into + lane * 16 + 1024, q + 1024);
+          cp_async16(into + lane * 16 + 1536, q + 1536);
         }
-        const uint32_t wa[4] = {ba[u].x, ba[u].y, ba[u].z, ba[u].w}, wb[4] = {bb[u].x, bb[u].y, bb[u].z, bb[u].w};
-        if (i + kAhead < n_kt) {
-          ba[u] = ld_stream16(qa + (int64_t)(i + kAhead) * 256);
-          bb[u] = ld_stream16(qb + (int64_t)(i + kAhead) * 256);
-        }
-        float fa[kGroups], fb[kGroups];
+        if (lane < (two ? 4 : 2) * kGroups) cp_async16(into + kPair * 1024 + lane * 16, sc);
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      fetched += kPair;
+      q += kPair * 1024;
+      sc += kPair * kGroups * 32;
+      into = into == ring + (kRing - 1) * kPair * kTileBytes ? ring : into + kPair * kTileBytes;
+    };
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          fa[g] = __half2float(sa[(int64_t)(i * kGroups + g) * 16]);
-          fb[g] = __half2float(sb[(int64_t)(i * kGroups + g) * 16]);
-        }
-        const uint32_t xoff = (uint32_t)(i - staged) * 256;
+    for (int i = 0; i < kRing - 1; ++i) fetch();
+    uint32_t xoff[MT];
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          float c[MT][4];
+    for (int m = 0; m < MT; ++m) xoff[m] = smem_u32(smem) + x_at + (kh * p.M + min(m * 8 + r, p.M - 1)) * kRowBytes + t * 8;
+    // one column tile: u of the stage at `at`, xo bytes into the token rows
+    auto column_tile = [&](uint32_t at, int u, uint32_t xo) {
+      const uint4 va = lds128(at + u * 1024 + lane * 16), vb = lds128(at + u * 1024 + lane * 16 + 512);
+      const uint32_t wa[4] = {va.x, va.y, va.z, va.w}, wb[4] = {vb.x, vb.y, vb.z, vb.w};
 #pragma unroll
-          for (int m = 0; m < MT; ++m) c[m][0] = c[m][1] = c[m][2] = c[m][3] = 0.f;
+      for (int g = 0; g < kGroups; ++g) {
+        const uint32_t s2 = lds32(at + kPair * 1024 + (u * kGroups + g) * 32 + r * 4);  // rows r and r + 8
+        const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&s2));
+        float c[MT][4];
 #pragma unroll
-          for (int s = g * GS; s < (g + 1) * GS; ++s) {
-            const uint32_t a[4] = {s & 1 ? codes2<2>(wa[s >> 1]) : codes2<0>(wa[s >> 1]),
-                                   s & 1 ? codes2<2>(wb[s >> 1]) : codes2<0>(wb[s >> 1]),
-                                   s & 1 ? codes2<3>(wa[s >> 1]) : codes2<1>(wa[s >> 1]),
-                                   s & 1 ? codes2<3>(wb[s >> 1]) : codes2<1>(wb[s >> 1])};
+        for (int m = 0; m < MT; ++m) c[m][0] = c[m][1] = c[m][2] = c[m][3] = 0.f;
 #pragma unroll
-            for (int m = 0; m < MT; ++m) {
-              uint32_t b0, b1;
-              asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(xrow[m] + xoff + s * 32));
-              mma_bf16(c[m], a, b0, b1);
-            }
-          }
+        for (int s = g * GS; s < (g + 1) * GS; ++s) {
+          const uint32_t a[4] = {s & 1 ? codes2<2>(wa[s >> 1], k) : codes2<0>(wa[s >> 1], k),
+                                 s & 1 ? codes2<2>(wb[s >> 1], k) : codes2<0>(wb[s >> 1], k),
+                                 s & 1 ? codes2<3>(wa[s >> 1], k) : codes2<1>(wa[s >> 1], k),
+                                 s & 1 ? codes2<3>(wb[s >> 1], k) : codes2<1>(wb[s >> 1], k)};
 #pragma unroll
           for (int m = 0; m < MT; ++m) {
-            acc[m][0] += fa[g] * c[m][0];
-            acc[m][1] += fa[g] * c[m][1];
-            acc[m][2] += fb[g] * c[m][2];
-            acc[m][3] += fb[g] * c[m][3];
+            uint32_t b0, b1;
+            asm volatile("ld.shared.v2.u32 {%0,%1}, [%2];" : "=r"(b0), "=r"(b1) : "r"(xoff[m] + xo + s * 32) : "memory");
+            mma_bf16(c[m], a, b0, b1);
           }
         }
+#pragma unroll
+        for (int m = 0; m < MT; ++m) {
+          acc[m][0] += f.x * c[m][0];
+          acc[m][1] += f.x * c[m][1];
+          acc[m][2] += f.y * c[m][2];
+          acc[m][3] += f.y * c[m][3];
+        }
       }
+    };
+    int buf = 0, parity = 0;
+    uint32_t at = ring;
+    for (int i0 = 0; i0 < mid; i0 += kXTiles) {
+      if (!mbar_wait(s_full + buf, parity, &s_abort)) give_up();
+      const uint32_t xo = buf * x_bytes;
+#pragma unroll
+      for (int j = 0; j < kXTiles; j += kPair) {
+        const int i = i0 + j;
+        if (i < n_kt) {
+          asm volatile("cp.async.wait_group %0;" ::"n"(kRing - 2) : "memory");
+          __syncwarp();  // the stage is there for every lane, and the one before it is free
+          fetch();
+#pragma unroll
+          for (int u = 0; u < kPair; ++u) {
+            if (i + u < n_kt) column_tile(at, u, xo + (j + u) * 256);
+          }
+          at = at == ring + (kRing - 1) * kPair * kTileBytes ? ring : at + kPair * kTileBytes;
+        }
+      }
+      __syncwarp();  // every lane has read the token rows
+      if (lane == 0) mbar_arrive(s_empty + buf);
+      if (++buf == 2) buf = 0, parity ^= 1;
     }
   }
-  // sums [token][row] in shared memory, then this CTA's share of the outputs
+  // sums [part][token][row] in shared memory, then this CTA's share of the outputs, four rows to a thread
   __syncthreads();
-  float* sums = reinterpret_cast<float*>(smem);
+  constexpr int kLd = kRowTiles * 16 + 4;
+  if (warp < kWarps) {
+    float* sums = reinterpret_cast<float*>(smem) + warp / kRowTiles * p.M * kLd + warp % kRowTiles * 16 + r;
 #pragma unroll
-  for (int m = 0; m < MT; ++m)
+    for (int m = 0; m < MT; ++m)
 #pragma unroll
-    for (int e = 0; e < 4; ++e) {
-      const int tok = m * 8 + 2 * t + (e & 1);
-      if (tok < p.M) sums[tok * kSumLd + warp * 16 + r + 8 * (e >> 1)] = acc[m][e];
-    }
+      for (int e = 0; e < 4; ++e) {
+        const int tok = m * 8 + 2 * t + (e & 1);
+        if (tok < p.M) sums[tok * kLd + 8 * (e >> 1)] = acc[m][e];
+      }
+  }
   if (S > 1) cluster_sync(); else __syncthreads();
   const uint32_t own = smem_u32(smem);
-  auto sum_at = [&](int tok, int row) {
-    if (S == 1) return sums[tok * kSumLd + row];
-    float v = 0.f;
-    for (int c = 0; c < S; ++c) v += ld_cluster(mapa_shared(own + (tok * kSumLd + row) * 4, c));
-    return v;
-  };
-  const int share = (p.M * outs + S - 1) / S;
-  for (int e = rank * share + tid; e < min(p.M * outs, (rank + 1) * share); e += kThreads) {
-    const int tok = e / outs, i = e % outs, n = n0 + i;
-    if (n >= p.n_out) continue;
-    float v = sum_at(tok, i);
-    if (p.bias) v += __bfloat162float(p.bias[n]);
-    if (p.swiglu) {
-      float u = sum_at(tok, kRows / 2 + i);
-      if (p.bias) u += __bfloat162float(p.bias[p.n_out + n]);
-      v = v / (1.f + __expf(-v)) * u;
+  constexpr int kUpAt = kRowTiles * 8;  // SwiGLU: the first up tile's place among the rows
+  auto sum_at = [&](int tok, int row) {  // four rows, all parts of all ranks
+    float4 v[8], w = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int h = 0; h < KH; ++h) {
+      const uint32_t a = own + ((h * p.M + tok) * kLd + row) * 4;
+#pragma unroll
+      for (int c = 0; c < 8; ++c) {
+        v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
+        if (c < S) v[c] = ld_cluster4(S > 1 ? mapa_shared(a, c) : a);
+      }
+#pragma unroll
+      for (int c = 0; c < 8; ++c) w.x += v[c].x, w.y += v[c].y, w.z += v[c].z, w.w += v[c].w;
     }
-    if (p.res) v += __bfloat162float(p.res[tok * p.rs + n]);
-    p.y[tok * p.ys + n] = __float2bfloat16(v);
+    return w;
+  };
+  const int quads = p.M * p.outs / 4, share = (quads + S - 1) / S;
+  for (int e = rank * share + tid; e < min(quads, (rank + 1) * share); e += kThreads) {
+    const int tok = e / (p.outs / 4), i = e % (p.outs / 4) * 4;
+    if (n0 + i >= p.n_out) continue;
+    const float4 v4 = sum_at(tok, i);
+    float v[4] = {v4.x, v4.y, v4.z, v4.w};
+    float u[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.swiglu) {  // up rows start `up` rows into their tiles: from the two aligned quads around them
+      const int o = up & 3;
+      const float4 a = sum_at(tok, kUpAt + ((up + i) & ~3));
+      float4 c = a;
+      if (o) c = sum_at(tok, kUpAt + ((up + i) & ~3) + 4);
+      u[0] = o == 0 ? a.x : o == 1 ? a.y : o == 2 ? a.z : a.w;
+      u[1] = o == 0 ? a.y : o == 1 ? a.z : o == 2 ? a.w : c.x;
+      u[2] = o == 0 ? a.z : o == 1 ? a.w : o == 2 ? c.x : c.y;
+      u[3] = o == 0 ? a.w : o == 1 ? c.x : o == 2 ? c.y : c.z;
+    }
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+      const int n = n0 + i + k;
+      if (n < p.n_out) {
+        if (p.bias) v[k] += __bfloat162float(p.bias[n]);
+        if (p.swiglu) {
+          if (p.bias) u[k] += __bfloat162float(p.bias[p.n_out + n]);
+          v[k] = v[k] / (1.f + __expf(-v[k])) * u[k];
+        }
+        if (p.res) v[k] += __bfloat162float(p.res[tok * p.rs + n]);
+        p.y[tok * p.ys + n] = __float2bfloat16(v[k]);
+      }
+    }
   }
   if (S > 1) cluster_sync();  // every CTA's sums are read before its shared memory goes
 }
 
-template <int MT, int GS>
+template <int MT, int GS, int KH>
 static void launch_linear(LinearParams& p, cudaStream_t st) {
-  const int sms = num_sms(current_device());
-  const int outs = p.swiglu ? kRows / 2 : kRows;
-  const int tiles = (p.n_out + outs - 1) / outs;
-  // columns are split until two CTAs an SM have work, while each keeps two column tiles
-  int S = 1;
-  while (S < 8 && tiles * S < 2 * sms && p.w.kt >= 4 * S) S *= 2;
-  const int per = (p.w.kt + S - 1) / S;
-  p.stage = std::max(1, std::min(per, (kStageBytes / p.M - 32) / 256));
-  const int smem = std::max(p.M * (p.stage * 256 + 32), p.M * kSumLd * 4);
+  constexpr int kRingBytes = kWarps * kRing * kPair * (1024 + 8 / GS * 32);
+  constexpr int kRowBytes = 4 / KH * 256 + 32;
+  static_assert(kRingBytes >= 128 * (MT * 8) * 4 + KH * MT * 8 * 16, "the sums fit the rings");
+  const int smem = kRingBytes + 2 * KH * p.M * kRowBytes;
+  constexpr int kSmem = kRingBytes + 2 * KH * MT * 8 * kRowBytes;
   static bool set[64] = {};
   const int dev = current_device();
   if (!set[dev]) {
-    AETHER_CUDA_CHECK(cudaFuncSetAttribute(linear_kernel<MT, GS>, cudaFuncAttributeMaxDynamicSharedMemorySize, kStageBytes));
+    AETHER_CUDA_CHECK(cudaFuncSetAttribute(linear_kernel<MT, GS, KH>, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
     set[dev] = true;
   }
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(tiles * S));
+  cfg.gridDim = dim3((unsigned)(p.tiles * p.S));
   cfg.blockDim = dim3(kThreads);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
-  cudaLaunchAttribute at{};
-  at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim = {(unsigned)S, 1, 1};
-  cfg.attrs = &at;
-  cfg.numAttrs = 1;
-  AETHER_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_kernel<MT, GS>, p));
+  cudaLaunchAttribute at[2] = {};
+  // the launch may begin while the kernel before it drains; this one waits for it before it touches memory
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  at[1].id = cudaLaunchAttributeClusterDimension;
+  at[1].val.clusterDim = {(unsigned)p.S, 1, 1};
+  cfg.attrs = at;
+  cfg.numAttrs = p.S > 1 ? 2 : 1;
+  AETHER_CUDA_CHECK(cudaLaunchKernelEx(&cfg, linear_kernel<MT, GS, KH>, p));
+}
+// Rows of a CTA and parts of the columns. An SM's fullest load is n CTAs of (column tiles + 4 for their start and end)
+// each; one alone leaves issue slots empty, two hide each other's waits.
+static int plan(LinearParams& p, int most_parts) {
+  const int sms = num_sms(current_device());
+  float best = 0.f;
+  int kh = 1;
+  for (int h = 1; h <= most_parts; ++h) {
+    const int rows = 128 / h;
+    const int outs = !p.swiglu ? rows : p.n_out % 16 == 0 ? rows / 2 : rows / 2 - 16;  // (see row_tile: one tile more)
+    const int tiles = (p.n_out + outs - 1) / outs;
+    for (int c = 1; c <= 8 && c <= p.w.kt; ++c) {
+      const int n = (tiles * c + sms - 1) / sms;
+      const float cost = (((p.w.kt + c - 1) / c + h - 1) / h + 4) * (n == 1 ? 0.7f : 0.5f * n);
+      if ((h == 1 && c == 1) || cost < best) best = cost, kh = h, p.S = c, p.outs = outs, p.tiles = tiles;
+    }
+  }
+  p.per = (p.w.kt + p.S - 1) / p.S;
+  return kh;
+}
+template <int MT, int GS>
+static void launch_parts(LinearParams& p, cudaStream_t st) {
+  if constexpr (MT == 8) {  // two parts' token rows would not fit beside three stages
+    plan(p, 1);
+    launch_linear<MT, GS, 1>(p, st);
+  } else {
+    if (plan(p, 2) == 1)
+      launch_linear<MT, GS, 1>(p, st);
+    else
+      launch_linear<MT, GS, 2>(p, st);
+  }
 }
 template <int MT>
 static void launch_group(LinearParams& p, cudaStream_t st) {
   if (p.w.gshift == 7)
-    launch_linear<MT, 8>(p, st);
+    launch_parts<MT, 8>(p, st);
   else if (p.w.gshift == 6)
-    launch_linear<MT, 4>(p, st);
+    launch_parts<MT, 4>(p, st);
   else
-    launch_linear<MT, 2>(p, st);
+    launch_parts<MT, 2>(p, st);
 }
 
 // out [N, K] bf16 = code * scale, for products of more rows than a decode
@@ -317,7 +431,7 @@ static Weight make_weight(const at::Tensor& q, const at::Tensor& s, int64_t N, i
                   reinterpret_cast<uintptr_t>(q.data_ptr()) % 16 == 0,
               what, ": q is contiguous CUDA int32 [ceil(N/16), ceil(K/128), 2, 32, 4]");
   TORCH_CHECK(s.device() == q.device() && s.scalar_type() == at::kHalf && s.is_contiguous() &&
-                  s.numel() == nt * (kt * 128 / group) * 16 && reinterpret_cast<uintptr_t>(s.data_ptr()) % 4 == 0,
+                  s.numel() == nt * (kt * 128 / group) * 16 && reinterpret_cast<uintptr_t>(s.data_ptr()) % 16 == 0,
               what, ": scales are contiguous float16 [ceil(N/16), ceil(K/128) * 128 / group, 8, 2] beside q");
   Weight w{};
   w.q = reinterpret_cast<const uint32_t*>(q.data_ptr<int>());
@@ -332,16 +446,19 @@ static Weight make_weight(const at::Tensor& q, const at::Tensor& s, int64_t N, i
 
 }  // namespace w4
 
-void linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group,
-               std::optional<at::Tensor> bias, std::optional<at::Tensor> residual, bool swiglu, at::Tensor y) {
+at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group,
+                     std::optional<at::Tensor> bias, std::optional<at::Tensor> residual, bool swiglu,
+                     std::optional<at::Tensor> out) {
   using namespace w4;
   LinearParams p{};
   p.w = make_weight(q, s, N, K, group, "linear_w4");
+  TORCH_CHECK(x.dim() == 2, "linear_w4: x is [M, K]");
   const int64_t M = x.size(0), n_out = swiglu ? N / 2 : N;
   TORCH_CHECK(!swiglu || N % 2 == 0, "linear_w4: SwiGLU takes an even number of rows (gate, then up)");
   TORCH_CHECK(x.device() == q.device() && x.scalar_type() == at::kBFloat16 && x.dim() == 2 && x.size(1) == K &&
                   x.stride(1) == 1,
               "linear_w4: x is bf16 [M, K] with unit inner stride, beside the weights");
+  const at::Tensor y = out && out->defined() ? *out : at::empty({M, n_out}, x.options());
   TORCH_CHECK(y.device() == q.device() && y.scalar_type() == at::kBFloat16 && y.dim() == 2 && y.size(0) == M &&
                   y.size(1) == n_out && (n_out == 1 || y.stride(1) == 1),
               "linear_w4: out is bf16 [M, N] (SwiGLU: [M, N / 2]) with unit inner stride, beside the weights");
@@ -359,8 +476,10 @@ void linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, i
     p.res = reinterpret_cast<const __nv_bfloat16*>(residual->data_ptr());
     p.rs = residual->stride(0);
   }
-  if (M == 0) return;
+  if (M == 0) return y;
   c10::cuda::CUDAGuard g(q.device());
+  // 16-byte copies: rows on 16-byte boundaries
+  if (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0 || (M > 1 && x.stride(0) % 8 != 0)) x = x.clone(at::MemoryFormat::Contiguous);
   p.x = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr());
   p.xs = x.stride(0);
   p.y = reinterpret_cast<__nv_bfloat16*>(y.data_ptr());
@@ -368,7 +487,7 @@ void linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, i
   p.M = (int)M;
   p.n_out = (int)n_out;
   p.swiglu = swiglu;
-  p.x_aligned = reinterpret_cast<uintptr_t>(p.x) % 16 == 0 && p.xs % 8 == 0;
+  p.status = device_status_word();
   auto st = at::cuda::getCurrentCUDAStream();
   if (M <= 8)
     launch_group<1>(p, st);
@@ -378,6 +497,7 @@ void linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, i
     launch_group<4>(p, st);
   else
     launch_group<8>(p, st);
+  return y;
 }
 
 void dequant_w4(at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group, at::Tensor out) {
