@@ -787,9 +787,9 @@ KV8_WORKSPACE = 16 << 20
 
 
 def kv8_workspace(device):
-    """Scratch of ``kv8_decode_attention`` (any shapes): zeroed once; every call
-    leaves its counters zero again. One call at a time may use it."""
-    return torch.zeros(KV8_WORKSPACE, dtype=torch.uint8, device=device)
+    """Scratch of ``kv8_decode_attention`` for any shapes. One call at a time may
+    use it."""
+    return torch.empty(KV8_WORKSPACE, dtype=torch.uint8, device=device)
 
 
 def _kv8_rows(x, name):

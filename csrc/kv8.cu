@@ -309,20 +309,20 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(GatherParams p) 
 // query heads) segments are laid end to end and cut into equal ranges, one for
 // each CTA (two of eight warps on an SM), so ragged batches fill the GPU; a
 // segment that one CTA holds whole is written at once, the parts of a cut one go
-// through the workspace and the last CTA to arrive joins them in order (a sum
-// that does not depend on who arrives when).
+// through the workspace to a second kernel, which joins them in order; it has its
+// prefix sums ready when the first one ends (joined by the last CTA to arrive,
+// 37 parts took 8 us of fences, waits and loads).
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
 constexpr int kMaxCtas = 512;       // parts: two for each CTA
-constexpr int kMaxSegments = 65536; // counters
 constexpr int kMaxSeqs = 8192;
 constexpr int kMinSteps = 2;        // of kWarps blocks: shorter ranges cost more to join than they save
+constexpr int kWholeKeys = 1024;    // page tables of at most so many positions: a CTA for each segment, none cut
 constexpr float kWeightBits = 10.f; // weights are at most 2^(10 + 4) in fp16
 constexpr int kPartFloats = 8 * 128 + 16;
-constexpr int64_t kWorkspaceBytes = (int64_t)kMaxSegments * 4 + (int64_t)kMaxCtas * 2 * kPartFloats * 4;
-// dynamic shared memory: [8 warps][8 heads][128] sums (the parts' weights [8][kMaxCtas] in the join), their M and
-// l, block records, prefix of steps
+constexpr int64_t kWorkspaceBytes = (int64_t)kMaxCtas * 2 * kPartFloats * 4;
+// dynamic shared memory: [8 warps][D / 16][32 lanes] 16-byte sums, their M and l, block records, prefix of steps
 constexpr int kSmemSums = kWarps * 8 * 128 * 4;
 constexpr int kSmemFixed = kSmemSums + 2 * kWarps * 8 * 4 + kWarps * 32 * 16;
 
@@ -335,9 +335,9 @@ struct AttnParams {
   Map m;
   const int* slot;
   const int* seqlen;
-  int* counters;  // [segments], zero between calls
-  float* parts;   // [CTAs][2][kPartFloats]
+  float* parts;   // [CTAs][2][kPartFloats]: a CTA's first segment's and its last one's, where they are cut
   int B, Hq, G, hg, window;  // G: query heads of a KV head; hg: groups of eight of them
+  int ctas;                  // of the attention kernel where segments are cut; 0: a CTA for each segment
   float scale_log2, cap_in, cap_out;  // cap_in = scale / softcap, cap_out = softcap * log2 e
   int* status;
 };
@@ -401,25 +401,10 @@ __device__ __forceinline__ void blocks_of(const AttnParams& p, int b, int& len, 
   count = len > 0 ? ((len + kBlock - 1) >> 4) - first : 0;
 }
 
-template <int D, bool CAP>
-__global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
-  constexpr int kKs = D / 16;   // k steps of S, m tiles of O
-  constexpr int kKl = D / 64;   // 16-byte loads of a key's row by a quad
-  extern __shared__ __align__(16) uint8_t smem[];
-  float* s_o = reinterpret_cast<float*>(smem);
-  float* s_m = s_o + kWarps * 8 * 128;  // [warps][8]
-  float* s_l = s_m + kWarps * 8;
-  int4* s_rec = reinterpret_cast<int4*>(s_l + kWarps * 8) + (threadIdx.x >> 5) * 32;  // this warp's
-  int* s_pre = reinterpret_cast<int*>(smem + kSmemFixed);  // [B + 1] steps before each sequence (one KV head)
-  __shared__ int s_warp[kWarps], s_flag;
+// s_pre[b]: steps (of kWarps blocks) before sequence b, for one KV head and group; returns their number. The host has
+// checked that all of them fit 30 bits.
+__device__ __forceinline__ int prefix_steps(const AttnParams& p, int* s_pre, int* s_warp) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  const int r = lane >> 2, t = lane & 3;
-  const int V = p.m.Hkv * p.hg;
-  const Consts konst{in_register(0x64646464u), in_register(0xe480e480u)};
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;");
-
-  // prefix of the steps (kWarps blocks) of every sequence; the host has checked that all of them fit 31 bits
   int carry = 0;
   for (int b0 = 0; b0 < p.B; b0 += kThreads) {
     int n = 0;
@@ -446,28 +431,75 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
     if (b0 + tid == p.B - 1) s_pre[p.B] = before + x;
     __syncthreads();
   }
-  const int total = carry * V;
-  const int per = max((total + (int)gridDim.x - 1) / (int)gridDim.x, kMinSteps);
-  int at = blockIdx.x * per;
-  const int end = min(total, at + per);
-  int b = 0;
-  if (at < end) {  // the last sequence that starts at or before `at`
-    int hi = p.B;
-    while (hi - b > 1) {
-      const int mid = (b + hi) >> 1;
-      if (s_pre[mid] * V <= at) b = mid; else hi = mid;
-    }
+  return carry;
+}
+__device__ __forceinline__ int steps_of_cta(int total, int ctas) { return max((total + ctas - 1) / ctas, kMinSteps); }
+// The last sequence that starts at or before step `at` of all.
+__device__ __forceinline__ int sequence_at(const int* s_pre, int B, int V, int at) {
+  int b = 0, hi = B;
+  while (hi - b > 1) {
+    const int mid = (b + hi) >> 1;
+    if (s_pre[mid] * V <= at) b = mid; else hi = mid;
+  }
+  while (s_pre[b + 1] == s_pre[b] || s_pre[b + 1] * V <= at) ++b;  // (not one without a key)
+  return b;
+}
+// The weight of a sum whose reference is m beside the largest reference: 0 for one of masked keys alone (l = 0).
+__device__ __forceinline__ float factor(float m, float l, float top) {
+  return m == -INFINITY ? (l == 0.f ? 0.f : 1.f) : ex2(m - top);
+}
+// Dims d and d + 1 of heads h and h + 1 (where there are so many) of an output row.
+__device__ __forceinline__ void write_out(__nv_bfloat16* y, int D, int h, int heads, const float4& a, float inv0, float inv1) {
+  if (h < heads) *reinterpret_cast<uint32_t*>(y) = pack_bf16(a.x * inv0, a.z * inv0);
+  if (h + 1 < heads) *reinterpret_cast<uint32_t*>(y + D) = pack_bf16(a.y * inv1, a.w * inv1);
+}
+
+template <int D, bool CAP>
+__global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
+  constexpr int kKs = D / 16;   // k steps of S, m tiles of O
+  constexpr int kKl = D / 64;   // 16-byte loads of a key's row by a quad
+  extern __shared__ __align__(16) uint8_t smem[];
+  float* s_o = reinterpret_cast<float*>(smem);
+  float* s_m = s_o + kWarps * 8 * 128;  // [warps][8]
+  float* s_l = s_m + kWarps * 8;
+  int4* s_rec = reinterpret_cast<int4*>(s_l + kWarps * 8) + (threadIdx.x >> 5) * 32;  // this warp's
+  int* s_pre = reinterpret_cast<int*>(smem + kSmemFixed);  // [B + 1] steps before each sequence (one KV head)
+  __shared__ int s_warp[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  const int r = lane >> 2, t = lane & 3;
+  const int V = p.m.Hkv * p.hg;
+  const Consts konst{in_register(0x64646464u), in_register(0xe480e480u)};
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+
+  int at = 0, end = 1, per = 1, b = blockIdx.x / V;
+  if (p.ctas > 0) {
+    const int total = prefix_steps(p, s_pre, s_warp) * V;
+    per = steps_of_cta(total, p.ctas);
+    at = blockIdx.x * per;
+    end = min(total, at + per);
+    if (at < end) b = sequence_at(s_pre, p.B, V, at);
   }
   while (at < end) {
-    while (s_pre[b + 1] == s_pre[b] || s_pre[b + 1] * V <= at) ++b;
-    const int steps = s_pre[b + 1] - s_pre[b];
-    const int off = at - s_pre[b] * V;
-    const int v = off / steps, st0 = off - v * steps;
-    const int st1 = min(steps, st0 + (end - at));
+    int len, lo, first, count, steps, v, st0, st1;
+    if (p.ctas > 0) {
+      while (s_pre[b + 1] == s_pre[b] || s_pre[b + 1] * V <= at) ++b;
+      steps = s_pre[b + 1] - s_pre[b];
+      const int off = at - s_pre[b] * V;
+      v = off / steps;
+      st0 = off - v * steps;
+      st1 = min(steps, st0 + (end - at));
+      blocks_of(p, b, len, lo, first, count);
+    } else {
+      v = blockIdx.x - b * V;
+      blocks_of(p, b, len, lo, first, count);
+      if (count == 0) break;
+      steps = (count + kWarps - 1) / kWarps;
+      st0 = 0;
+      st1 = steps;
+    }
     const int hk = v / p.hg, h0 = hk * p.G + (v - hk * p.hg) * 8;
     const int heads = min(8, p.G - (v - hk * p.hg) * 8);
-    int len, lo, first, count;
-    blocks_of(p, b, len, lo, first, count);
     const int slot = p.slot[b];
     const int blk0 = first + st0 * kWarps + warp;              // this warp's blocks: blk0, blk0 + kWarps, ...
     const int blk1 = min(first + count, first + st1 * kWarps);
@@ -503,24 +535,28 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
     };
     // Records of this warp's next 32 blocks: page, key scale, log2 and inverse of the value scale. The first block's
     // codes are asked for as soon as its page is known, beside the scales.
-    auto fill = [&](int i0) {
-      int page = -1;
+    int rpage;
+    float rks, rvs;
+    auto fetch_records = [&](int i0) {
+      rpage = -1;
       const int pos = (blk0 + (i0 + lane) * kWarps) << 4;
-      if (i0 + lane < n_blk) page = page_of(p.m, slot, pos, p.status);
-      const int64_t base = block_base(max(__shfl_sync(0xffffffffu, page, 0), 0), blk0 + i0 * kWarps);
+      if (i0 + lane < n_blk) rpage = page_of(p.m, slot, pos, p.status);
+      const int64_t base = block_base(max(__shfl_sync(0xffffffffu, rpage, 0), 0), blk0 + i0 * kWarps);
       load_k(base);
       load_v(base);
-      float ks = 0.f, vs = 0.f;
-      if (page >= 0) {
-        const int64_t so = scale_offset(p.m, page, hk, pos & ((1 << p.m.shift) - 1));
-        ks = p.k.scale[so];
-        vs = p.v.scale[so];
+      rks = rvs = 0.f;
+      if (rpage >= 0) {
+        const int64_t so = scale_offset(p.m, rpage, hk, pos & ((1 << p.m.shift) - 1));
+        rks = p.k.scale[so];
+        rvs = p.v.scale[so];
       }
-      vs = vs < 6.2e-33f ? 6.2e-33f : vs;  // (a NaN stays)
+    };
+    auto store_records = [&]() {
+      const float vs = rvs < 6.2e-33f ? 6.2e-33f : rvs;  // (a NaN stays)
       __syncwarp();
       // an unusable page has weights of zero
-      s_rec[lane] = make_int4(max(page, 0), __float_as_int(ks), __float_as_int(page >= 0 ? log2f(vs) : -INFINITY),
-                              __float_as_int(page >= 0 ? 1.f / vs : 0.f));
+      s_rec[lane] = make_int4(max(rpage, 0), __float_as_int(rks), __float_as_int(rpage >= 0 ? log2f(vs) : -INFINITY),
+                              __float_as_int(rpage >= 0 ? 1.f / vs : 0.f));
       __syncwarp();
     };
     uint4 qraw[kKl][2];  // head r, dims 16 t .. of each 64
@@ -531,7 +567,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) qraw[i][j] = *reinterpret_cast<const uint4*>(qr + i * 64 + j * 8);
     }
-    if (n_blk > 0) fill(0);
+    if (n_blk > 0) fetch_records(0);
 
     // q as the B operand
     uint32_t qb[kKs][2];
@@ -573,7 +609,8 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
 
     for (int i0 = 0; i0 < n_blk; i0 += 32) {
       const int nb = min(32, n_blk - i0);
-      if (i0 > 0) fill(i0);
+      if (i0 > 0) fetch_records(i0);
+      store_records();
       for (int i = 0; i < nb; ++i) {
         const int4 rec = s_rec[i];
         const int pos = (blk0 + (i0 + i) * kWarps) << 4;
@@ -652,137 +689,147 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
         if (i + 1 < nb) load_v(base);
       }
     }
-    // join the warps: o[k][0], [2] are dims (D / 8) r + 2 k and + 1 of head 2 t; [1], [3] of head 2 t + 1
+    // Join the warps. o[k] is dims (D / 8) r + 2 k and the next (elements 0, 1 and 2, 3) of heads 2 t and 2 t + 1; sums
+    // and parts keep that order, [k][lane] 16 bytes each, and warp k joins its slice.
 #pragma unroll
     for (int s = 4; s < 32; s <<= 1) {
       l0 += __shfl_xor_sync(0xffffffffu, l0, s);
       l1 += __shfl_xor_sync(0xffffffffu, l1, s);
     }
     if (r == 0) {
-      s_m[warp * 8 + 2 * t] = m0;
-      s_m[warp * 8 + 2 * t + 1] = m1;
-      s_l[warp * 8 + 2 * t] = l0;
-      s_l[warp * 8 + 2 * t + 1] = l1;
+      *reinterpret_cast<float2*>(s_m + warp * 8 + 2 * t) = make_float2(m0, m1);
+      *reinterpret_cast<float2*>(s_l + warp * 8 + 2 * t) = make_float2(l0, l1);
     }
+    float4* sums = reinterpret_cast<float4*>(s_o);
 #pragma unroll
-    for (int k = 0; k < kKs; ++k) {
-      float* d = s_o + (warp * 8 + 2 * t) * D + (D / 8) * r + 2 * k;
-      *reinterpret_cast<float2*>(d) = make_float2(o[k][0], o[k][2]);
-      *reinterpret_cast<float2*>(d + D) = make_float2(o[k][1], o[k][3]);
-    }
+    for (int k = 0; k < kKs; ++k) sums[(warp * kKs + k) * 32 + lane] = make_float4(o[k][0], o[k][1], o[k][2], o[k][3]);
     __syncthreads();
     const bool whole = st0 == 0 && st1 == steps;
-    const int seg0 = s_pre[b] * V + v * steps;  // the segment's first step
-    const int cta0 = seg0 / per;
-    float* part = p.parts + ((int64_t)blockIdx.x * 2 + (cta0 == (int)blockIdx.x ? 1 : 0)) * kPartFloats;
-    constexpr int kPer = 8 * D / kThreads;  // consecutive dims of one head for each thread
-    {
-      const int g = tid * kPer / D, d = tid * kPer % D;
-      float mm = -INFINITY;
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, s_m[w * 8 + g]);
-      float ll = 0.f, acc[kPer];
-#pragma unroll
-      for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
+    if (warp < kKs) {
+      float mm0 = -INFINITY, mm1 = -INFINITY, ll0 = 0.f, ll1 = 0.f;
+      float2 mw[kWarps];
 #pragma unroll
       for (int w = 0; w < kWarps; ++w) {
-        const float mw = s_m[w * 8 + g];
-        const float f = mw == -INFINITY ? (s_l[w * 8 + g] == 0.f ? 0.f : 1.f) : ex2(mw - mm);  // l is 0 or NaN
-        ll += f * s_l[w * 8 + g];
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[e] += f * s_o[(w * 8 + g) * D + d + e];
+        mw[w] = *reinterpret_cast<const float2*>(s_m + w * 8 + 2 * t);
+        mm0 = fmaxf(mm0, mw[w].x);
+        mm1 = fmaxf(mm1, mw[w].y);
       }
+      float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+      for (int w = 0; w < kWarps; ++w) {
+        const float2 lw = *reinterpret_cast<const float2*>(s_l + w * 8 + 2 * t);
+        const float f0 = factor(mw[w].x, lw.x, mm0), f1 = factor(mw[w].y, lw.y, mm1);
+        const float4 x = sums[(w * kKs + warp) * 32 + lane];
+        ll0 += f0 * lw.x;
+        ll1 += f1 * lw.y;
+        acc.x += f0 * x.x;
+        acc.y += f1 * x.y;
+        acc.z += f0 * x.z;
+        acc.w += f1 * x.w;
+      }
+      const int h = 2 * t;
       if (whole) {
-        if (g < heads) {
-          const float inv = ll == 0.f ? 0.f : 1.f / ll;
-          __nv_bfloat16* y = p.out + (int64_t)b * p.o_rs + (int64_t)(h0 + g) * D + d;
-#pragma unroll
-          for (int e = 0; e < kPer; e += 2)
-            *reinterpret_cast<uint32_t*>(y + e) = pack_bf16(acc[e] * inv, acc[e + 1] * inv);
-        }
+        write_out(p.out + (int64_t)b * p.o_rs + (int64_t)(h0 + h) * D + (D / 8) * r + 2 * warp, D, h, heads, acc,
+                  ll0 == 0.f ? 0.f : 1.f / ll0, ll1 == 0.f ? 0.f : 1.f / ll1);
       } else {
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) part[g * D + d + e] = acc[e];
-        if (d == 0) {
-          part[8 * D + g] = mm;
-          part[8 * D + 8 + g] = ll;
+        const bool begins = s_pre[b] * V + v * steps >= (int)blockIdx.x * per;  // the segment's first part
+        float* part = p.parts + ((int64_t)blockIdx.x * 2 + begins) * kPartFloats;
+        reinterpret_cast<float4*>(part)[warp * 32 + lane] = acc;
+        if (warp == 0 && r == 0) {
+          *reinterpret_cast<float2*>(part + 8 * D + h) = make_float2(mm0, mm1);
+          *reinterpret_cast<float2*>(part + 8 * D + 8 + h) = make_float2(ll0, ll1);
         }
       }
     }
-    if (!whole) {
-      const int np = (seg0 + steps - 1) / per - cta0 + 1;
-      __threadfence();
-      __syncthreads();
-      if (tid == 0) s_flag = atomicAdd(p.counters + b * V + v, 1) == np - 1;
-      __syncthreads();
-      if (s_flag) {
-        __threadfence();
-        auto part_of = [&](int i) { return p.parts + ((int64_t)(cta0 + i) * 2 + (i == 0 ? 1 : 0)) * kPartFloats; };
-        constexpr int kBatch = 16;  // parts in flight
-        const int g = tid * kPer / D, d = tid * kPer % D;
-        float pv[kBatch][kPer];
-        auto load_parts = [&](int i0) {
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i) {
-            const float* src = part_of(min(i0 + i, np - 1)) + g * D + d;
-            if constexpr (kPer == 4) {
-              const float4 q4 = __ldcg(reinterpret_cast<const float4*>(src));
-              pv[i][0] = q4.x, pv[i][1] = q4.y, pv[i][2] = q4.z, pv[i][3] = q4.w;
-            } else {
-              const float2 q2 = __ldcg(reinterpret_cast<const float2*>(src));
-              pv[i][0] = q2.x, pv[i][1] = q2.y;
-            }
-          }
-        };
-        load_parts(0);
-        {  // warp h: the parts' weights for head h, 2^(M_i - M) / l
-          float* wgt = s_o + warp * kMaxCtas;
-          float mm = -INFINITY, ll = 0.f;
-          for (int i = lane; i < np; i += 32) {
-            const float mi = __ldcg(part_of(i) + 8 * D + warp), li = __ldcg(part_of(i) + 8 * D + 8 + warp);
-            const float mn = fmaxf(mm, mi);
-            const float f = mi == -INFINITY ? (li == 0.f ? 0.f : 1.f) : 1.f;
-            ll = ll * (mm == -INFINITY ? 1.f : ex2(mm - mn)) + li * f * (mi == -INFINITY ? 1.f : ex2(mi - mn));
-            mm = mn;
-            wgt[i] = f == 0.f ? -INFINITY : mi;
-          }
-          const float ml = mm;
-          mm = warp_max(mm);
-          ll = warp_sum(ll * (ml == -INFINITY ? 1.f : ex2(ml - mm)));
-          const float inv = ll == 0.f ? 0.f : 1.f / ll;
-          for (int i = lane; i < np; i += 32) wgt[i] = (wgt[i] == -INFINITY ? 0.f : ex2(wgt[i] - mm)) * inv;
-        }
-        __syncthreads();
-        const float* wgt = s_o + g * kMaxCtas;
-        float acc[kPer];
-#pragma unroll
-        for (int e = 0; e < kPer; ++e) acc[e] = 0.f;
-        for (int i0 = 0; i0 < np; i0 += kBatch) {
-          if (i0 > 0) load_parts(i0);
-#pragma unroll
-          for (int i = 0; i < kBatch; ++i)
-            if (i0 + i < np) {
-#pragma unroll
-              for (int e = 0; e < kPer; ++e) acc[e] += wgt[i0 + i] * pv[i][e];
-            }
-        }
-        if (g < heads) {
-          __nv_bfloat16* y = p.out + (int64_t)b * p.o_rs + (int64_t)(h0 + g) * D + d;
-#pragma unroll
-          for (int e = 0; e < kPer; e += 2) *reinterpret_cast<uint32_t*>(y + e) = pack_bf16(acc[e], acc[e + 1]);
-        }
-        if (tid == 0) p.counters[b * V + v] = 0;  // ready for the next call
-      }
-    }
+    if (p.ctas == 0) break;
     __syncthreads();  // the sums are free again
     at += st1 - st0;
   }
   // sequences without a key: zero rows
-  for (b = blockIdx.x; b < p.B; b += gridDim.x) {
-    if (s_pre[b + 1] != s_pre[b]) continue;
+  const int nb = p.ctas > 0 ? p.B : (blockIdx.x % V == 0 ? blockIdx.x / V + 1 : 0);
+  for (b = p.ctas > 0 ? blockIdx.x : blockIdx.x / V; b < nb; b += gridDim.x) {
+    int len, lo, first, count;
+    blocks_of(p, b, len, lo, first, count);
+    if (count > 0) continue;
     for (int i = tid; i < p.Hq * D / 8; i += kThreads)
       *reinterpret_cast<uint4*>(p.out + (int64_t)b * p.o_rs + i * 8) = make_uint4(0, 0, 0, 0);
   }
+}
+
+// Joins the segment that the boundary between CTAs blockIdx.x and the next cuts, if it is that segment's first one:
+// o = sum_i 2^(M_i - M) o_i / sum_i 2^(M_i - M) l_i, the parts in order. Latency is all there is: everything but the
+// parts is known before the attention kernel ends (which has waited for the inputs to be complete before it let
+// this one begin), and a batch of parts is in flight at once.
+template <int D>
+__global__ void __launch_bounds__(kThreads) join_kernel(AttnParams p) {
+  constexpr int kKs = D / 16;
+  extern __shared__ __align__(16) uint8_t smem[];
+  int* s_pre = reinterpret_cast<int*>(smem);
+  __shared__ int s_warp[kWarps];
+  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
+  const int V = p.m.Hkv * p.hg;
+  const int total = prefix_steps(p, s_pre, s_warp) * V;
+  const int per = steps_of_cta(total, p.ctas);
+  const int cut = ((int)blockIdx.x + 1) * per;
+  bool mine = cut < total && warp < kKs;
+  int b = 0, v = 0, np = 0;
+  if (mine) {
+    b = sequence_at(s_pre, p.B, V, cut);
+    const int steps = s_pre[b + 1] - s_pre[b];
+    v = (cut - s_pre[b] * V) / steps;
+    const int seg0 = s_pre[b] * V + v * steps;
+    mine = seg0 < cut && seg0 / per == (int)blockIdx.x;
+    np = (seg0 + steps - 1) / per - (int)blockIdx.x + 1;
+  }
+  asm volatile("griddepcontrol.wait;" ::: "memory");
+  asm volatile("griddepcontrol.launch_dependents;");
+  if (!mine) return;
+  // part i: this CTA's last segment, then each following CTA's first
+  const float* parts = p.parts + (int64_t)blockIdx.x * 2 * kPartFloats;
+  constexpr int kBatch = 12;
+  float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
+  float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+  for (int i0 = 0; i0 < np; i0 += kBatch) {
+    float2 pm[kBatch], pl[kBatch];
+    float4 po[kBatch];
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      const int n = min(i0 + i, np - 1);
+      const float* part = parts + (2 * n + (n == 0 ? 1 : 0)) * kPartFloats;
+      pm[i] = *reinterpret_cast<const float2*>(part + 8 * D + 2 * t);
+      pl[i] = *reinterpret_cast<const float2*>(part + 8 * D + 8 + 2 * t);
+      po[i] = reinterpret_cast<const float4*>(part)[warp * 32 + lane];
+    }
+    float t0 = m0, t1 = m1;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      t0 = fmaxf(t0, pm[i].x);
+      t1 = fmaxf(t1, pm[i].y);
+    }
+    const float a0 = factor(m0, l0, t0), a1 = factor(m1, l1, t1);
+    l0 *= a0;
+    l1 *= a1;
+    acc.x *= a0;
+    acc.y *= a1;
+    acc.z *= a0;
+    acc.w *= a1;
+    m0 = t0;
+    m1 = t1;
+#pragma unroll
+    for (int i = 0; i < kBatch; ++i) {
+      if (i0 + i >= np) break;
+      const float f0 = factor(pm[i].x, pl[i].x, t0), f1 = factor(pm[i].y, pl[i].y, t1);
+      l0 += f0 * pl[i].x;
+      l1 += f1 * pl[i].y;
+      acc.x += f0 * po[i].x;
+      acc.y += f1 * po[i].y;
+      acc.z += f0 * po[i].z;
+      acc.w += f1 * po[i].w;
+    }
+  }
+  const int hk = v / p.hg, g0 = (v - hk * p.hg) * 8, h = 2 * t;
+  write_out(p.out + (int64_t)b * p.o_rs + (int64_t)(hk * p.G + g0 + h) * D + (D / 8) * r + 2 * warp, D, h, min(8, p.G - g0),
+            acc, l0 == 0.f ? 0.f : 1.f / l0, l1 == 0.f ? 0.f : 1.f / l1);
 }
 
 // ------------------------------------------------------------------ host
@@ -961,8 +1008,7 @@ at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::
   check_ints(seqlen, kc, B, "kv8_decode_attention: seqlen [B]");
   TORCH_CHECK(window >= 0 && window < (int64_t(1) << 31) && softcap >= 0, "kv8_decode_attention: window and softcap");
   const int64_t G = Hq / Hkv, hg = (G + 7) / 8;
-  TORCH_CHECK(B <= kMaxSeqs && B * Hkv * hg <= kMaxSegments,
-              "kv8_decode_attention: at most 8192 sequences and 65536 (sequence, KV head, eight query heads)");
+  TORCH_CHECK(B <= kMaxSeqs, "kv8_decode_attention: at most 8192 sequences");
   TORCH_CHECK(workspace.device() == kc.device() && workspace.scalar_type() == at::kByte && workspace.is_contiguous() &&
                   workspace.numel() >= kWorkspaceBytes && reinterpret_cast<uintptr_t>(workspace.data_ptr()) % 16 == 0,
               "kv8_decode_attention: workspace from kv8_workspace on the cache's device");
@@ -978,8 +1024,7 @@ at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::
   p.m = make_map(kc, page_table);
   p.slot = slot.data_ptr<int>();
   p.seqlen = seqlen.data_ptr<int>();
-  p.counters = reinterpret_cast<int*>(workspace.data_ptr());
-  p.parts = reinterpret_cast<float*>(p.counters + kMaxSegments);
+  p.parts = reinterpret_cast<float*>(workspace.data_ptr());
   p.B = (int)B;
   p.Hq = (int)Hq;
   p.G = (int)G;
@@ -995,10 +1040,13 @@ at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::
   if (window > 0) keys = std::min<int64_t>(keys, window + kBlock);
   const int64_t most = B * Hkv * hg * std::max<int64_t>(1, (keys + kWarps * kBlock - 1) / (kWarps * kBlock));
   TORCH_CHECK(most < (int64_t(1) << 30), "kv8_decode_attention: the page table's positions times sequences and heads");
-  const int grid = (int)std::min<int64_t>(std::min(2 * num_sms(current_device()), kMaxCtas), most);
+  // short tables: a CTA for each segment; else equal ranges for two CTAs an SM
+  const int grid = keys <= kWholeKeys ? (int)(B * Hkv * hg)
+                                      : (int)std::min<int64_t>(std::min(2 * num_sms(current_device()), kMaxCtas), most);
+  p.ctas = keys <= kWholeKeys ? 0 : grid;
   const int smem = kSmemFixed + ((int)B + 1) * 4;
   auto st = at::cuda::getCurrentCUDAStream();
-  auto launch = [&](auto kernel, bool* set) {
+  auto launch = [&](auto kernel, auto join, bool* set) {
     const int dev = current_device();
     if (!set[dev]) {
       AETHER_CUDA_CHECK(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize,
@@ -1006,16 +1054,17 @@ at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::
       set[dev] = true;
     }
     launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, st, p);
+    if (p.ctas > 1) launch_pdl(join, dim3(grid - 1), dim3(kThreads), ((int)B + 1) * 4, st, p);
   };
   static bool set[4][64] = {};
   if (D == 128 && softcap > 0)
-    launch(attn_kernel<128, true>, set[0]);
+    launch(attn_kernel<128, true>, join_kernel<128>, set[0]);
   else if (D == 128)
-    launch(attn_kernel<128, false>, set[1]);
+    launch(attn_kernel<128, false>, join_kernel<128>, set[1]);
   else if (softcap > 0)
-    launch(attn_kernel<64, true>, set[2]);
+    launch(attn_kernel<64, true>, join_kernel<64>, set[2]);
   else
-    launch(attn_kernel<64, false>, set[3]);
+    launch(attn_kernel<64, false>, join_kernel<64>, set[3]);
   return out;
 }
 
