@@ -90,10 +90,10 @@ struct AppendParams {
 // as NaN. With row_start, unit u belongs to the sequence b whose first unit
 // row_start[b] / 16 + 2 b is the last one not after u: a sequence of n rows
 // touches at most n / 16 + 1.875 blocks, so these ranges never overlap.
-// Bound by the bytes of qkv and out: a warp has a block's 4 KB of one head in
-// flight, and the warps of a CTA walk over the heads of one block of tokens, so
-// that its rows of cos and sin come from L1 after the first. A few tokens get a
-// warp for each head instead (one token a block: latency is all there is).
+// q heads need no block: a warp turns kTok tokens of one head after another and
+// keeps the tokens' angles in registers. Bound by the bytes of qkv and out while
+// blocks are many; a few tokens are spread over more CTAs (latency is all there
+// is).
 constexpr int kAppendWarps = 8;
 
 template <int D>
@@ -104,7 +104,6 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) append_kernel(AppendPara
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int H = p.Hq + 2 * p.m.Hkv;
   int b, j, r0, n;
   if (p.row_start == nullptr) {
     b = blockIdx.x;
@@ -136,39 +135,48 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) append_kernel(AppendPara
   if (page < 0) return;
   const int c = (lane % kLanes) * 8, sub = lane / kLanes;
   const int row = base & ((1 << p.m.shift) - 1);
-  for (int h = blockIdx.y * kAppendWarps + warp; h < H; h += gridDim.y * kAppendWarps) {
-    const bool is_q = h < p.Hq, is_v = h >= p.Hq + p.m.Hkv;
+  const int gw = blockIdx.y * kAppendWarps + warp, W = gridDim.y * kAppendWarps;
+  // y = x rotated by position t's angles, dims c .. and D / 2 + c ..
+  auto angles = [&](int t, float (&cs)[8], float (&sn)[8]) {
+    const float4* cp = reinterpret_cast<const float4*>(p.cos_t + (int64_t)t * (D / 2) + c);
+    const float4* sp = reinterpret_cast<const float4*>(p.sin_t + (int64_t)t * (D / 2) + c);
+    const float4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
+    cs[0] = c0.x, cs[1] = c0.y, cs[2] = c0.z, cs[3] = c0.w, cs[4] = c1.x, cs[5] = c1.y, cs[6] = c1.z, cs[7] = c1.w;
+    sn[0] = s0.x, sn[1] = s0.y, sn[2] = s0.z, sn[3] = s0.w, sn[4] = s1.x, sn[5] = s1.y, sn[6] = s1.z, sn[7] = s1.w;
+  };
+  auto rotate = [&](float (&a)[8], float (&bb)[8], const float (&cs)[8], const float (&sn)[8]) {
+#pragma unroll
+    for (int e = 0; e < 8; ++e) {
+      const float x1 = a[e], x2 = bb[e];
+      a[e] = __fsub_rn(__fmul_rn(x1, cs[e]), __fmul_rn(x2, sn[e]));
+      bb[e] = __fadd_rn(__fmul_rn(x2, cs[e]), __fmul_rn(x1, sn[e]));
+    }
+  };
+  // k and v heads: the whole block at once
+  for (int h = gw; h < 2 * p.m.Hkv; h += W) {
+    const bool is_v = h >= p.m.Hkv;
     const Pool& pool = is_v ? p.v : p.k;
-    const int hk = h - p.Hq - (is_v ? p.m.Hkv : 0);
-    uint8_t* codes = pool.codes + code_offset(p.m, page, max(hk, 0), row);
-    float* scale = pool.scale + scale_offset(p.m, page, max(hk, 0), row);
-    const float s_old = !is_q && lo > base ? *scale : 0.f;
+    const int hk = is_v ? h - p.m.Hkv : h;
+    uint8_t* codes = pool.codes + code_offset(p.m, page, hk, row);
+    float* scale = pool.scale + scale_offset(p.m, page, hk, row);
+    const float s_old = lo > base ? *scale : 0.f;
     uint4 xa[kIt], xb[kIt];
 #pragma unroll
     for (int i = 0; i < kIt; ++i) {
       const int t = base + i * kTok + sub;
       if (t >= lo && t < hi) {
-        const __nv_bfloat16* x = p.qkv + (int64_t)(r0 + (t - pos)) * p.rs + (int64_t)h * D + c;
+        const __nv_bfloat16* x = p.qkv + (int64_t)(r0 + (t - pos)) * p.rs + (int64_t)(p.Hq + h) * D + c;
         xa[i] = *reinterpret_cast<const uint4*>(x);
         xb[i] = *reinterpret_cast<const uint4*>(x + D / 2);
       }
     }
-    // dims c .. and D / 2 + c .. of position t, rotated
     auto value = [&](int i, int t, float (&a)[8], float (&bb)[8]) {
       dec::unpack8(xa[i], a);
       dec::unpack8(xb[i], bb);
       if (is_v) return;
-      const float4* cp = reinterpret_cast<const float4*>(p.cos_t + (int64_t)t * (D / 2) + c);
-      const float4* sp = reinterpret_cast<const float4*>(p.sin_t + (int64_t)t * (D / 2) + c);
-      const float4 c0 = __ldg(cp), c1 = __ldg(cp + 1), s0 = __ldg(sp), s1 = __ldg(sp + 1);
-      const float cs[8] = {c0.x, c0.y, c0.z, c0.w, c1.x, c1.y, c1.z, c1.w};
-      const float sn[8] = {s0.x, s0.y, s0.z, s0.w, s1.x, s1.y, s1.z, s1.w};
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float x1 = a[e], x2 = bb[e];
-        a[e] = __fsub_rn(__fmul_rn(x1, cs[e]), __fmul_rn(x2, sn[e]));
-        bb[e] = __fadd_rn(__fmul_rn(x2, cs[e]), __fmul_rn(x1, sn[e]));
-      }
+      float cs[8], sn[8];
+      angles(t, cs, sn);
+      rotate(a, bb, cs, sn);
     };
     uint32_t top = 0;
 #pragma unroll
@@ -178,17 +186,14 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) append_kernel(AppendPara
       float a[8], bb[8];
       value(i, t, a, bb);
       if (!is_v) {
-        __nv_bfloat16* o = p.out + (int64_t)(r0 + (t - pos)) * p.os + (int64_t)h * D + c;
+        __nv_bfloat16* o = p.out + (int64_t)(r0 + (t - pos)) * p.os + (int64_t)(p.Hq + h) * D + c;
         *reinterpret_cast<uint4*>(o) = dec::pack8(a);
         *reinterpret_cast<uint4*>(o + D / 2) = dec::pack8(bb);
       }
-      if (!is_q) {
 #pragma unroll
-        for (int e = 0; e < 8; ++e)
-          top = max(top, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(bb[e]) & 0x7fffffffu));
-      }
+      for (int e = 0; e < 8; ++e)
+        top = max(top, max(__float_as_uint(a[e]) & 0x7fffffffu, __float_as_uint(bb[e]) & 0x7fffffffu));
     }
-    if (is_q) continue;
     top = __reduce_max_sync(0xffffffffu, top);
     // 2^-100: a block of zeros gets a tiny scale, and 1 / s stays finite
     const float s_new = __fdiv_rn(__uint_as_float(max(top, 0x0d800000u)), 127.f);
@@ -224,6 +229,38 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) append_kernel(AppendPara
       *reinterpret_cast<uint2*>(d + D / 2) = make_uint2(w[2], w[3]);
     }
   }
+  // q heads: kTok tokens of a head at a time, four heads in flight, the tokens' angles kept from head to head
+  const int i_lo = (lo - base) / kTok, ni = (hi - 1 - base) / kTok - i_lo + 1, step = W / ni;
+  if (gw >= step * ni) return;
+  const int t = base + (i_lo + gw % ni) * kTok + sub;
+  const bool in = t >= lo && t < hi;
+  const int64_t tok = r0 + (in ? t - pos : lo - pos);
+  float cs[8], sn[8];
+  angles(in ? t : lo, cs, sn);
+  const __nv_bfloat16* x = p.qkv + tok * p.rs + c;
+  __nv_bfloat16* o = p.out + tok * p.os + c;
+  constexpr int kHeads = 4;
+  for (int h = gw / ni; h < p.Hq; h += kHeads * step) {
+    uint4 xa[kHeads], xb[kHeads];
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k)
+      if (h + k * step < p.Hq) {
+        xa[k] = *reinterpret_cast<const uint4*>(x + (h + k * step) * D);
+        xb[k] = *reinterpret_cast<const uint4*>(x + (h + k * step) * D + D / 2);
+      }
+#pragma unroll
+    for (int k = 0; k < kHeads; ++k)
+      if (h + k * step < p.Hq) {
+        float a[8], bb[8];
+        dec::unpack8(xa[k], a);
+        dec::unpack8(xb[k], bb);
+        rotate(a, bb, cs, sn);
+        if (in) {
+          *reinterpret_cast<uint4*>(o + (h + k * step) * D) = dec::pack8(a);
+          *reinterpret_cast<uint4*>(o + (h + k * step) * D + D / 2) = dec::pack8(bb);
+        }
+      }
+  }
 }
 
 // ------------------------------------------------------------------ gather
@@ -242,7 +279,7 @@ struct GatherParams {
 // the bytes moved; a position's heads are one run of the output, and 128 bytes
 // of a head's row one line of the pool.
 constexpr int kGatherThreads = 256;
-constexpr int kGatherRows = 4;
+constexpr int kGatherRows = 2;
 
 // four codes of w times s
 __device__ __forceinline__ uint2 four(uint32_t w, float s) {
@@ -403,10 +440,11 @@ __device__ __forceinline__ void blocks_of(const AttnParams& p, int b, int& len, 
 
 // s_pre[b]: steps (of kWarps blocks) before sequence b, for one KV head and group; returns their number. The host has
 // checked that all of them fit 30 bits.
+template <int kSides = 1>  // of kThreads threads
 __device__ __forceinline__ int prefix_steps(const AttnParams& p, int* s_pre, int* s_warp) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int carry = 0;
-  for (int b0 = 0; b0 < p.B; b0 += kThreads) {
+  for (int b0 = 0; b0 < p.B; b0 += kThreads * kSides) {
     int n = 0;
     if (b0 + tid < p.B) {
       int len, lo, first, count;
@@ -423,7 +461,7 @@ __device__ __forceinline__ int prefix_steps(const AttnParams& p, int* s_pre, int
     __syncthreads();
     int before = carry;
 #pragma unroll
-    for (int w = 0; w < kWarps; ++w) {
+    for (int w = 0; w < kWarps * kSides; ++w) {
       if (w < warp) before += s_warp[w];
       carry += s_warp[w];
     }
@@ -760,18 +798,21 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
 // o = sum_i 2^(M_i - M) o_i / sum_i 2^(M_i - M) l_i, the parts in order. Latency is all there is: everything but the
 // parts is known before the attention kernel ends (which has waited for the inputs to be complete before it let
 // this one begin), and a batch of parts is in flight at once.
+constexpr int kJoinSides = 2;  // halves of the parts, side by side
+
 template <int D>
-__global__ void __launch_bounds__(kThreads) join_kernel(AttnParams p) {
+__global__ void __launch_bounds__(kThreads * kJoinSides) join_kernel(AttnParams p) {
   constexpr int kKs = D / 16;
   extern __shared__ __align__(16) uint8_t smem[];
   int* s_pre = reinterpret_cast<int*>(smem);
-  __shared__ int s_warp[kWarps];
-  const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31, r = lane >> 2, t = lane & 3;
+  __shared__ int s_warp[kWarps * kJoinSides];
+  __shared__ float4 s_acc[kThreads], s_ml[kThreads];
+  const int tid = threadIdx.x, side = tid / kThreads, warp = tid / 32 % kWarps, lane = tid & 31, r = lane >> 2, t = lane & 3;
   const int V = p.m.Hkv * p.hg;
-  const int total = prefix_steps(p, s_pre, s_warp) * V;
+  const int total = prefix_steps<kJoinSides>(p, s_pre, s_warp) * V;
   const int per = steps_of_cta(total, p.ctas);
   const int cut = ((int)blockIdx.x + 1) * per;
-  bool mine = cut < total && warp < kKs;
+  bool mine = cut < total;
   int b = 0, v = 0, np = 0;
   if (mine) {
     b = sequence_at(s_pre, p.B, V, cut);
@@ -784,17 +825,18 @@ __global__ void __launch_bounds__(kThreads) join_kernel(AttnParams p) {
   asm volatile("griddepcontrol.wait;" ::: "memory");
   asm volatile("griddepcontrol.launch_dependents;");
   if (!mine) return;
-  // part i: this CTA's last segment, then each following CTA's first
+  // part i: this CTA's last segment, then each following CTA's first; a side takes its half of them
   const float* parts = p.parts + (int64_t)blockIdx.x * 2 * kPartFloats;
-  constexpr int kBatch = 12;
+  const int half = (np + 1) / 2, n0 = side * half, n1 = min(np, n0 + half);
+  constexpr int kBatch = 10;
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-  for (int i0 = 0; i0 < np; i0 += kBatch) {
+  for (int i0 = n0; i0 < n1 && warp < kKs; i0 += kBatch) {
     float2 pm[kBatch], pl[kBatch];
     float4 po[kBatch];
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      const int n = min(i0 + i, np - 1);
+      const int n = min(i0 + i, n1 - 1);
       const float* part = parts + (2 * n + (n == 0 ? 1 : 0)) * kPartFloats;
       pm[i] = *reinterpret_cast<const float2*>(part + 8 * D + 2 * t);
       pl[i] = *reinterpret_cast<const float2*>(part + 8 * D + 8 + 2 * t);
@@ -817,7 +859,7 @@ __global__ void __launch_bounds__(kThreads) join_kernel(AttnParams p) {
     m1 = t1;
 #pragma unroll
     for (int i = 0; i < kBatch; ++i) {
-      if (i0 + i >= np) break;
+      if (i0 + i >= n1) break;
       const float f0 = factor(pm[i].x, pl[i].x, t0), f1 = factor(pm[i].y, pl[i].y, t1);
       l0 += f0 * pl[i].x;
       l1 += f1 * pl[i].y;
@@ -827,6 +869,18 @@ __global__ void __launch_bounds__(kThreads) join_kernel(AttnParams p) {
       acc.w += f1 * po[i].w;
     }
   }
+  if (side == 1) {
+    s_acc[tid - kThreads] = acc;
+    s_ml[tid - kThreads] = make_float4(m0, m1, l0, l1);
+  }
+  __syncthreads();
+  if (side == 1 || warp >= kKs) return;
+  const float4 o = s_acc[tid], ml = s_ml[tid];
+  const float t0 = fmaxf(m0, ml.x), t1 = fmaxf(m1, ml.y);
+  const float a0 = factor(m0, l0, t0), a1 = factor(m1, l1, t1), c0 = factor(ml.x, ml.z, t0), c1 = factor(ml.y, ml.w, t1);
+  l0 = l0 * a0 + ml.z * c0;
+  l1 = l1 * a1 + ml.w * c1;
+  acc = make_float4(acc.x * a0 + o.x * c0, acc.y * a1 + o.y * c1, acc.z * a0 + o.z * c0, acc.w * a1 + o.w * c1);
   const int hk = v / p.hg, g0 = (v - hk * p.hg) * 8, h = 2 * t;
   write_out(p.out + (int64_t)b * p.o_rs + (int64_t)(hk * p.G + g0 + h) * D + (D / 8) * r + 2 * warp, D, h, min(8, p.G - g0),
             acc, l0 == 0.f ? 0.f : 1.f / l0, l1 == 0.f ? 0.f : 1.f / l1);
@@ -1054,7 +1108,7 @@ at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::
       set[dev] = true;
     }
     launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, st, p);
-    if (p.ctas > 1) launch_pdl(join, dim3(grid - 1), dim3(kThreads), ((int)B + 1) * 4, st, p);
+    if (p.ctas > 1) launch_pdl(join, dim3(grid - 1), dim3(kThreads * kJoinSides), ((int)B + 1) * 4, st, p);
   };
   static bool set[4][64] = {};
   if (D == 128 && softcap > 0)
