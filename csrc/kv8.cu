@@ -97,7 +97,7 @@ struct AppendParams {
 constexpr int kAppendWarps = 8;
 
 template <int D>
-__global__ void __launch_bounds__(kAppendWarps * 32, 3) append_kernel(AppendParams p) {
+__global__ void __launch_bounds__(kAppendWarps * 32, 2) append_kernel(AppendParams p) {
   constexpr int kLanes = D / 16;            // lanes of one token: 8 + 8 dims each
   constexpr int kTok = 32 / kLanes;         // tokens side by side
   constexpr int kIt = kBlock / kTok;
@@ -229,7 +229,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) append_kernel(AppendPara
       *reinterpret_cast<uint2*>(d + D / 2) = make_uint2(w[2], w[3]);
     }
   }
-  // q heads: kTok tokens of a head at a time, four heads in flight, the tokens' angles kept from head to head
+  // q heads: kTok tokens of a head at a time, seven heads in flight, the tokens' angles kept from head to head
   const int i_lo = (lo - base) / kTok, ni = (hi - 1 - base) / kTok - i_lo + 1, step = W / ni;
   if (gw >= step * ni) return;
   const int t = base + (i_lo + gw % ni) * kTok + sub;
@@ -239,7 +239,7 @@ __global__ void __launch_bounds__(kAppendWarps * 32, 3) append_kernel(AppendPara
   angles(in ? t : lo, cs, sn);
   const __nv_bfloat16* x = p.qkv + tok * p.rs + c;
   __nv_bfloat16* o = p.out + tok * p.os + c;
-  constexpr int kHeads = 4;
+  constexpr int kHeads = 7;
   for (int h = gw / ni; h < p.Hq; h += kHeads * step) {
     uint4 xa[kHeads], xb[kHeads];
 #pragma unroll
@@ -798,18 +798,17 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
 // o = sum_i 2^(M_i - M) o_i / sum_i 2^(M_i - M) l_i, the parts in order. Latency is all there is: everything but the
 // parts is known before the attention kernel ends (which has waited for the inputs to be complete before it let
 // this one begin), and a batch of parts is in flight at once.
-constexpr int kJoinSides = 2;  // halves of the parts, side by side
-
-template <int D>
-__global__ void __launch_bounds__(kThreads * kJoinSides) join_kernel(AttnParams p) {
+// kSides: halves of the parts, side by side
+template <int D, int kSides>
+__global__ void __launch_bounds__(kThreads * kSides) join_kernel(AttnParams p) {
   constexpr int kKs = D / 16;
   extern __shared__ __align__(16) uint8_t smem[];
   int* s_pre = reinterpret_cast<int*>(smem);
-  __shared__ int s_warp[kWarps * kJoinSides];
-  __shared__ float4 s_acc[kThreads], s_ml[kThreads];
+  __shared__ int s_warp[kWarps * kSides];
+  __shared__ float4 s_acc[kSides == 2 ? kThreads : 1], s_ml[kSides == 2 ? kThreads : 1];
   const int tid = threadIdx.x, side = tid / kThreads, warp = tid / 32 % kWarps, lane = tid & 31, r = lane >> 2, t = lane & 3;
   const int V = p.m.Hkv * p.hg;
-  const int total = prefix_steps<kJoinSides>(p, s_pre, s_warp) * V;
+  const int total = prefix_steps<kSides>(p, s_pre, s_warp) * V;
   const int per = steps_of_cta(total, p.ctas);
   const int cut = ((int)blockIdx.x + 1) * per;
   bool mine = cut < total;
@@ -827,8 +826,8 @@ __global__ void __launch_bounds__(kThreads * kJoinSides) join_kernel(AttnParams 
   if (!mine) return;
   // part i: this CTA's last segment, then each following CTA's first; a side takes its half of them
   const float* parts = p.parts + (int64_t)blockIdx.x * 2 * kPartFloats;
-  const int half = (np + 1) / 2, n0 = side * half, n1 = min(np, n0 + half);
-  constexpr int kBatch = 10;
+  const int half = (np + kSides - 1) / kSides, n0 = side * half, n1 = min(np, n0 + half);
+  constexpr int kBatch = kSides == 2 ? 10 : 8;
   float m0 = -INFINITY, m1 = -INFINITY, l0 = 0.f, l1 = 0.f;
   float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
   for (int i0 = n0; i0 < n1 && warp < kKs; i0 += kBatch) {
@@ -869,18 +868,21 @@ __global__ void __launch_bounds__(kThreads * kJoinSides) join_kernel(AttnParams 
       acc.w += f1 * po[i].w;
     }
   }
-  if (side == 1) {
-    s_acc[tid - kThreads] = acc;
-    s_ml[tid - kThreads] = make_float4(m0, m1, l0, l1);
+  if constexpr (kSides == 2) {
+    if (side == 1) {
+      s_acc[tid - kThreads] = acc;
+      s_ml[tid - kThreads] = make_float4(m0, m1, l0, l1);
+    }
+    __syncthreads();
+    if (side == 1) return;
+    const float4 o = s_acc[tid], ml = s_ml[tid];
+    const float t0 = fmaxf(m0, ml.x), t1 = fmaxf(m1, ml.y);
+    const float a0 = factor(m0, l0, t0), a1 = factor(m1, l1, t1), c0 = factor(ml.x, ml.z, t0), c1 = factor(ml.y, ml.w, t1);
+    l0 = l0 * a0 + ml.z * c0;
+    l1 = l1 * a1 + ml.w * c1;
+    acc = make_float4(acc.x * a0 + o.x * c0, acc.y * a1 + o.y * c1, acc.z * a0 + o.z * c0, acc.w * a1 + o.w * c1);
   }
-  __syncthreads();
-  if (side == 1 || warp >= kKs) return;
-  const float4 o = s_acc[tid], ml = s_ml[tid];
-  const float t0 = fmaxf(m0, ml.x), t1 = fmaxf(m1, ml.y);
-  const float a0 = factor(m0, l0, t0), a1 = factor(m1, l1, t1), c0 = factor(ml.x, ml.z, t0), c1 = factor(ml.y, ml.w, t1);
-  l0 = l0 * a0 + ml.z * c0;
-  l1 = l1 * a1 + ml.w * c1;
-  acc = make_float4(acc.x * a0 + o.x * c0, acc.y * a1 + o.y * c1, acc.z * a0 + o.z * c0, acc.w * a1 + o.w * c1);
+  if (warp >= kKs) return;
   const int hk = v / p.hg, g0 = (v - hk * p.hg) * 8, h = 2 * t;
   write_out(p.out + (int64_t)b * p.o_rs + (int64_t)(hk * p.G + g0 + h) * D + (D / 8) * r + 2 * warp, D, h, min(8, p.G - g0),
             acc, l0 == 0.f ? 0.f : 1.f / l0, l1 == 0.f ? 0.f : 1.f / l1);
@@ -1100,6 +1102,9 @@ at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::
   p.ctas = keys <= kWholeKeys ? 0 : grid;
   const int smem = kSmemFixed + ((int)B + 1) * 4;
   auto st = at::cuda::getCurrentCUDAStream();
+  // many parts a segment: two halves of them side by side (37 parts: 3 us less); else the smaller CTA, which finds room
+  // as soon as one of the attention kernel's ends (64 x 4096: 3 us less)
+  const int sides = p.ctas > 12 * B * Hkv * hg ? 2 : 1;
   auto launch = [&](auto kernel, auto join, bool* set) {
     const int dev = current_device();
     if (!set[dev]) {
@@ -1108,17 +1113,17 @@ at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::
       set[dev] = true;
     }
     launch_pdl(kernel, dim3(grid), dim3(kThreads), smem, st, p);
-    if (p.ctas > 1) launch_pdl(join, dim3(grid - 1), dim3(kThreads * kJoinSides), ((int)B + 1) * 4, st, p);
+    if (p.ctas > 1) launch_pdl(join, dim3(grid - 1), dim3(kThreads * sides), ((int)B + 1) * 4, st, p);
   };
   static bool set[4][64] = {};
   if (D == 128 && softcap > 0)
-    launch(attn_kernel<128, true>, join_kernel<128>, set[0]);
+    launch(attn_kernel<128, true>, sides == 2 ? join_kernel<128, 2> : join_kernel<128, 1>, set[0]);
   else if (D == 128)
-    launch(attn_kernel<128, false>, join_kernel<128>, set[1]);
+    launch(attn_kernel<128, false>, sides == 2 ? join_kernel<128, 2> : join_kernel<128, 1>, set[1]);
   else if (softcap > 0)
-    launch(attn_kernel<64, true>, join_kernel<64>, set[2]);
+    launch(attn_kernel<64, true>, sides == 2 ? join_kernel<64, 2> : join_kernel<64, 1>, set[2]);
   else
-    launch(attn_kernel<64, false>, join_kernel<64>, set[3]);
+    launch(attn_kernel<64, false>, sides == 2 ? join_kernel<64, 2> : join_kernel<64, 1>, set[3]);
   return out;
 }
 
