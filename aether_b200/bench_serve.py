@@ -9,6 +9,7 @@ events, p50 over --ttft-reps); decode tok/s = batch * steps / device time of
 ``steps`` graph replays. One JSON line per (config, batch).
 
     python -m aether_b200.bench_serve --model 7b --batches 1,16,64
+    python -m aether_b200.bench_serve --model 7b --w4 128 --kv-bits 8   # 4-bit projections, 8-bit paged KV cache
     torchrun --nproc-per-node N -m aether_b200.bench_serve --model 7b --tp N
 """
 from __future__ import annotations
@@ -21,7 +22,7 @@ import statistics
 import torch
 
 from . import _ext
-from .models.qwen import QwenConfig, QwenModel
+from .models.qwen import QwenConfig, QwenModel, QwenWeights
 
 
 class EmulatedTP:
@@ -85,15 +86,21 @@ def events():
     return torch.cuda.Event(enable_timing=True), torch.cuda.Event(enable_timing=True)
 
 
-def run(model_name: str, batches, prompt: int, new_tokens: int, ttft_reps: int, tp=None, rank0=True):
+def run(model_name: str, batches, prompt: int, new_tokens: int, ttft_reps: int, tp=None, rank0=True, w4=0, kv_bits=16):
     cfg = QwenConfig.qwen25_7b() if model_name == "7b" else QwenConfig.qwen25_1_5b()
     maxb = max(batches)
     dev = torch.device("cuda", torch.cuda.current_device())
-    m = QwenModel(cfg, device=dev, seed=0, max_batch=maxb, max_seq=4096, tp=tp)
+    weights = QwenWeights(cfg, dev).quantize_w4(w4) if w4 else None
+    pages = maxb * 4096 // 64 + 1 if kv_bits == 8 else 0
+    m = QwenModel(cfg, device=dev, seed=0, max_batch=maxb, max_seq=4096, tp=tp, weights=weights, kv_pages=pages,
+                  kv_bits=kv_bits)
     g = torch.Generator(device="cpu").manual_seed(7)
     out = []
     for B in batches:
         prompts = torch.randint(0, cfg.vocab, (B, prompt), generator=g).to(dev)
+        for r in range(B if m.paged else 0):
+            m.cache.release(r)
+            m.cache.ensure(r, prompt + new_tokens)
         # warm-up: prefill + graph capture
         m.prefill(prompts)
         tok = torch.zeros(B, dtype=torch.long, device=dev)
@@ -131,6 +138,7 @@ def run(model_name: str, batches, prompt: int, new_tokens: int, ttft_reps: int, 
             "batch": B, "prompt": prompt, "new_tokens": new_tokens, "value": B / (ms_step / 1e3), "unit": "tokens/s",
             "ms_per_decode_step": ms_step, "ttft_p50_ms": statistics.median(tt), "ttft_all_ms": tt,
             "decode_splits": m.decode_splits, "graph": True, "dtype": "bf16",
+            "weights": f"4-bit, groups of {w4}" if w4 else "bf16", "kv_bits": kv_bits,
             "data": "synthetic uniform-random prompts, random-init weights",
             "kv_cache_gb": m.cache.bytes() / 1e9,
         }
@@ -151,6 +159,9 @@ def main():
     ap.add_argument("--tp", type=int, default=1)
     ap.add_argument("--emulate-tp", type=int, default=0,
                     help="one GPU runs one TP rank's shards without communication (the TP compute floor)")
+    ap.add_argument("--w4", type=int, default=0, metavar="GROUP",
+                    help="4-bit projections with a scale for each GROUP columns (32, 64 or 128; one GPU)")
+    ap.add_argument("--kv-bits", type=int, default=16, choices=[8, 16], help="8: paged KV cache in 8 bits")
     args = ap.parse_args()
     _ext.C()
     batches = [int(b) for b in (args.batches or ("1,8,32" if args.model == "1.5b" else "1,16,64")).split(",")]
@@ -166,7 +177,7 @@ def main():
         info = D.init()
         tp = TensorParallel(info)
         rank0 = info.is_main
-    run(args.model, batches, prompt, args.new_tokens, args.ttft_reps, tp, rank0)
+    run(args.model, batches, prompt, args.new_tokens, args.ttft_reps, tp, rank0, args.w4, args.kv_bits)
     if tp is not None and hasattr(tp, "close"):
         tp.close()
 

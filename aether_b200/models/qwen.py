@@ -222,6 +222,19 @@ class QwenWeights:
         if not cfg.tie_embeddings:
             self.lm_head = None  # each rank streams only its slice
 
+    def quantize_w4(self, group: int = 128) -> "QwenWeights":
+        """Replaces the four projections of every layer by 4-bit codes with a
+        scale for each ``group`` columns (``ops.functional.W4Weight``); decode
+        multiplies them as they are, prefill expands them before each GEMM.
+        Embeddings, LM head, norms and biases stay bf16."""
+        if self.tp_size > 1:
+            raise ValueError("4-bit projections serve one GPU (the TP shards are bf16)")
+        for ws in (self.wqkv, self.wo, self.wgu, self.wd):
+            for i, t in enumerate(ws):
+                if not isinstance(t, F.W4Weight):
+                    ws[i] = F.quantize_w4(t if isinstance(t, torch.Tensor) else t.bf16(), group)
+        return self
+
     @staticmethod
     def shard(full: "QwenWeights", tp_rank: int, tp_size: int, device) -> "QwenWeights":
         """One rank's shard of full (e.g. GGUF- or HF-loaded) weights, in the
@@ -278,10 +291,11 @@ class QwenModel:
 
     def __init__(self, cfg: QwenConfig, device="cuda", seed: int = 0, max_batch: int = 64, max_seq: int | None = None,
                  weights: QwenWeights | None = None, tp=None, decode_splits: int = 0, kv_pages: int = 0,
-                 page_size: int = 64):
+                 page_size: int = 64, kv_bits: int = 16):
         """kv_pages > 0 selects the paged KV cache (``serving.kv.PagedKVCache``)
         with that many pages of ``page_size`` tokens shared by all sequences;
-        otherwise every batch slot owns a contiguous max_seq cache."""
+        otherwise every batch slot owns a contiguous max_seq cache. kv_bits 8
+        (paged only) holds the pages in 8 bits (``serving.kv.Paged8KVCache``)."""
         self.cfg = cfg
         self.device = torch.device(device)
         self.tp = tp
@@ -297,17 +311,21 @@ class QwenModel:
         self.max_batch = max_batch
         self.max_seq = max_seq or cfg.max_seq
         # one extra slot absorbs the K/V writes of padded batch rows
+        if kv_bits not in (8, 16) or (kv_bits == 8 and kv_pages <= 0):
+            raise ValueError("kv_bits: 16, or 8 with kv_pages > 0")
+        self.kv8 = kv_bits == 8
         if kv_pages > 0:
-            from ..serving.kv import PagedKVCache
+            from ..serving.kv import Paged8KVCache, PagedKVCache
 
-            self.cache = PagedKVCache(cfg.n_layers, self.hkv, cfg.head_dim, kv_pages, page_size, max_batch + 1,
-                                      self.max_seq, self.device)
+            self.cache = (Paged8KVCache if self.kv8 else PagedKVCache)(cfg.n_layers, self.hkv, cfg.head_dim, kv_pages, page_size, max_batch + 1,
+                                                                       self.max_seq, self.device)
             self.page_table = self.cache.table
         else:
             self.cache = KVCache(cfg, self.hkv, max_batch + 1, self.max_seq, self.device)
             self.page_table = None
         self.paged = self.page_table is not None
-        self.scratch_slot = max_batch
+        # padded batch rows: the scratch slot and one key, or (8-bit cache) no slot and no key
+        self.scratch_slot, self._pad_len = (-1, 0) if self.kv8 else (max_batch, 1)
         cos, sin = ref.rope_tables(self.max_seq, cfg.head_dim, cfg.rope_theta, device=self.device)
         self.cos, self.sin = cos.contiguous(), sin.contiguous()
         # per-layer flex attention parameters: window and RoPE tables
@@ -326,7 +344,9 @@ class QwenModel:
         self.decode_splits = decode_splits or self._auto_splits(1)  # the most any batch size uses
         import os as _os
         # the fused decode epilogue has no slot for Qwen3's q/k norm
-        self.fused_decode = _os.environ.get("AETHER_UNFUSED_DECODE", "0") != "1" and not cfg.qk_norm
+        # (and none for an 8-bit cache or 4-bit projections, whose kernels have epilogues of their own)
+        self.fused_decode = (_os.environ.get("AETHER_UNFUSED_DECODE", "0") != "1" and not cfg.qk_norm
+                             and not self.kv8 and not isinstance(self.w.wqkv[0], F.W4Weight))
         # QKV (bias + RoPE + KV append) and SwiGLU finished inside their decode GEMMs (opt-in:
         # measured on a B200 the tile finisher serialises in the GEMM tail -- Qwen2.5-7B TP1
         # batch 64: 7.43 ms per step against 5.72 with the separate finalize kernels; batch 1
@@ -397,6 +417,8 @@ class QwenModel:
             # per-tile K-block counters of the fused-epilogue GEMMs (they return to zero)
             "tiles": torch.zeros(max(qkv_w // 128, self.f // 64) + 1, dtype=torch.int32, device=dev),
         }
+        if self.kv8 and dev.type == "cuda":
+            self.buf["kv8"] = F.kv8_workspace(dev)
         self._want_logits = False
 
     # ------------------------------------------------------------------ prefill
@@ -414,15 +436,23 @@ class QwenModel:
             slots = torch.arange(B, dtype=torch.int32, device=dev)
         T = B * S
         pos = (torch.arange(S, dtype=torch.int32, device=dev) + start_pos).repeat(B)
-        slot_t = slots.to(dev, torch.int32).repeat_interleave(S)
+        slots = slots.to(dev, torch.int32)
+        slot_t = slots.repeat_interleave(S)
+        if self.kv8:
+            first = torch.full((B,), start_pos, dtype=torch.int32, device=dev)
+            row_start = torch.arange(B + 1, dtype=torch.int32, device=dev) * S
         x = F.embedding(w.embed, tokens.to(dev).reshape(-1))
         row = (self.hq + 2 * self.hkv) * D
         for i in range(cfg.n_layers):
             h, _, _ = F.rmsnorm(x, w.attn_norm[i], cfg.norm_eps)
             qkv = F.gemm(h, self._mat(w.wqkv[i]), bias=w.bqkv[i])
             self._qk_norm(i, qkv)
-            F.rope_kv_append(qkv, pos, slot_t, *self.rope_cs[i], self.cache.k[i], self.cache.v[i], self.hq,
-                             self.hkv, D, page_table=self.page_table)
+            if self.kv8:
+                F.rope_kv8_append(qkv, first, slots, *self.rope_cs[i], *self.cache.layer(i), self.page_table, self.hq,
+                                  row_start=row_start)
+            else:
+                F.rope_kv_append(qkv, pos, slot_t, *self.rope_cs[i], self.cache.k[i], self.cache.v[i], self.hq,
+                                 self.hkv, D, page_table=self.page_table)
             q = qkv.view(B, S, row)[:, :, : self.hq * D].view(B, S, self.hq, D)
             if start_pos == 0:
                 k = qkv.view(B, S, row)[:, :, self.hq * D : (self.hq + self.hkv) * D].view(B, S, self.hkv, D)
@@ -431,7 +461,14 @@ class QwenModel:
                                    softcap=self.softcap)
             else:
                 Lk = start_pos + S
-                if self.paged:
+                if self.kv8:  # the prefix from its 8 bits, this chunk as computed
+                    kc, ks, vc, vs = self.cache.layer(i)
+                    k = F.gather_kv8(kc, ks, self.page_table, slots, 0, Lk)
+                    v = F.gather_kv8(vc, vs, self.page_table, slots, 0, Lk)
+                    new = qkv.view(B, S, row)[:, :, self.hq * D :].view(B, S, 2, self.hkv, D)
+                    k[:, start_pos:] = new[:, :, 0]
+                    v[:, start_pos:] = new[:, :, 1]
+                elif self.paged:
                     rows = [int(r) for r in slots.tolist()]
                     k = torch.stack([F.gather_kv(self.cache.k[i], r, Lk, self.page_table) for r in rows])
                     v = torch.stack([F.gather_kv(self.cache.v[i], r, Lk, self.page_table) for r in rows])
@@ -681,7 +718,8 @@ class QwenModel:
                       b["next"][:B], logits, self.cache.k[0], self.page_table, rank, world, timeout)
 
     def _decode_body_unfused(self, B: int) -> None:
-        """Decode step with separate norm / RoPE / combine kernels (13 per layer)."""
+        """Decode step with separate norm / RoPE / combine kernels (13 per layer;
+        8 with 4-bit projections and an 8-bit cache)."""
         cfg, w, b = self.cfg, self.w, self.buf
         D = cfg.head_dim
         x, x2, h = b["x"][:B], b["x2"][:B], b["h"][:B]
@@ -690,20 +728,24 @@ class QwenModel:
         x.copy_(F.embedding(w.embed, b["tok"][:B]))
         for i in range(cfg.n_layers):
             F.rmsnorm_into(x, w.attn_norm[i], h, cfg.norm_eps)
-            F.skinny_gemm(h, self._mat(w.wqkv[i]), acc)
-            F.skinny_finalize(acc, qkv, bias=w.bqkv[i])
+            self._project(h, w.wqkv[i], acc, qkv, bias=w.bqkv[i])
             self._qk_norm(i, qkv)
-            F.rope_kv_append(qkv, pos, slot, *self.rope_cs[i], self.cache.k[i], self.cache.v[i], self.hq, self.hkv, D,
-                             page_table=self.page_table)
-            F.decode_attention(qkv, self.cache.k[i], self.cache.v[i], slot, seqlen, o, self.hq, self.scale,
-                               self._auto_splits(B), b["part_o"], b["part_lse"], page_table=self.page_table,
-                               window=self.win[i], softcap=self.softcap)
+            if self.kv8:
+                kv = self.cache.layer(i)
+                F.rope_kv8_append(qkv, pos, slot, *self.rope_cs[i], *kv, self.page_table, self.hq)
+                F.kv8_decode_attention(qkv, *kv, self.page_table, slot, seqlen, self.hq, self.scale, out=o,
+                                       workspace=b.get("kv8"), window=self.win[i], softcap=self.softcap)
+            else:
+                F.rope_kv_append(qkv, pos, slot, *self.rope_cs[i], self.cache.k[i], self.cache.v[i], self.hq, self.hkv,
+                                 D, page_table=self.page_table)
+                F.decode_attention(qkv, self.cache.k[i], self.cache.v[i], slot, seqlen, o, self.hq, self.scale,
+                                   self._auto_splits(B), b["part_o"], b["part_lse"], page_table=self.page_table,
+                                   window=self.win[i], softcap=self.softcap)
             if self._push_for(B):
                 F.skinny_gemm(o, self._mat(w.wo[i]), acc)
                 self.tp.push_reduce(acc, x2, res=x)
             elif self.tp is None:
-                F.skinny_gemm(o, self._mat(w.wo[i]), acc)
-                F.skinny_finalize(acc, x2, res=x)
+                self._project(o, w.wo[i], acc, x2, res=x)
             else:
                 racc = self.tp.reduce_gemm(o, self._mat(w.wo[i]), 2 * i)
                 F.skinny_finalize(racc, x2, res=x, wait=self._tp_wait())
@@ -711,6 +753,15 @@ class QwenModel:
             self._decode_ffn(i, h, x2, x, act, acc)
         F.rmsnorm_into(x, w.final_norm, h, cfg.norm_eps)
         self._decode_head(B, h, acc)
+
+    def _project(self, x, w, acc, y, bias=None, res=None) -> None:
+        """y = x w^T (+ bias) (+ res) on the decode rows: a 4-bit weight in one
+        kernel, any other through the fp32 accumulator."""
+        if isinstance(w, F.W4Weight):
+            F.linear_w4(x, w, bias=bias, residual=res, out=y)
+            return
+        F.skinny_gemm(x, self._mat(w), acc)
+        F.skinny_finalize(acc, y, bias=bias, res=res)
 
     def _tp_wait(self):
         return self.tp.finalize_wait() if self.tp is not None else None
@@ -731,14 +782,16 @@ class QwenModel:
     def _decode_ffn(self, i, h, x2, x, act, acc) -> None:
         """x = x2 + FFN(h) on the decode rows (static buffers)."""
         w = self.w
-        F.skinny_gemm(h, self._mat(w.wgu[i]), acc)
-        F.skinny_finalize(acc, act, swiglu=True)
+        if isinstance(w.wgu[i], F.W4Weight):
+            F.linear_w4(h, w.wgu[i], swiglu=True, out=act)
+        else:
+            F.skinny_gemm(h, self._mat(w.wgu[i]), acc)
+            F.skinny_finalize(acc, act, swiglu=True)
         if self._push_for(h.shape[0]):
             F.skinny_gemm(act, self._mat(w.wd[i]), acc)
             self.tp.push_reduce(acc, x, res=x2)
         elif self.tp is None:
-            F.skinny_gemm(act, self._mat(w.wd[i]), acc)
-            F.skinny_finalize(acc, x, res=x2)
+            self._project(act, w.wd[i], acc, x, res=x2)
         else:
             racc = self.tp.reduce_gemm(act, self._mat(w.wd[i]), 2 * i + 1)
             F.skinny_finalize(racc, x, res=x2, wait=self._tp_wait())
@@ -788,7 +841,7 @@ class QwenModel:
         if Bb > B:  # padded rows decode into spare slots and are ignored
             b["tok"][B:Bb].zero_()
             b["pos"][B:Bb].zero_()
-            b["seqlen"][B:Bb].fill_(1)
+            b["seqlen"][B:Bb].fill_(self._pad_len)
             b["slot"][B:Bb].fill_(self.scratch_slot)
         if use_graph and self.device.type == "cuda":
             if (Bb, want_logits) not in self._graphs:

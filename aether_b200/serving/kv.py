@@ -93,14 +93,17 @@ class PagedKVCache:
         assert page_size & (page_size - 1) == 0, "page size must be a power of two"
         self.page_size, self.rows, self.max_seq = page_size, rows, max_seq
         self.max_pages = (max_seq + page_size - 1) // page_size
-        shape = (num_pages, page_size, n_kv_heads, head_dim)
-        self.k = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(n_layers)]
-        self.v = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(n_layers)]
+        self._make_pools(n_layers, num_pages, n_kv_heads, head_dim, device)
         # page 0 is the scratch page: unused table entries and padded batch rows point at it
         self.alloc = PageAllocator(num_pages, page_size, reserved=1)
         self.table = torch.zeros(rows, self.max_pages, dtype=torch.int32, device=device)
         self.pages: list = [[] for _ in range(rows)]
         self.device = torch.device(device)
+
+    def _make_pools(self, n_layers: int, num_pages: int, n_kv_heads: int, head_dim: int, device) -> None:
+        shape = (num_pages, self.page_size, n_kv_heads, head_dim)
+        self.k = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(n_layers)]
+        self.v = [torch.zeros(shape, dtype=torch.bfloat16, device=device) for _ in range(n_layers)]
 
     def bytes(self) -> int:
         return sum(t.numel() * 2 for t in self.k + self.v)
@@ -148,3 +151,28 @@ class PagedKVCache:
             self.alloc.release(p)
         self.pages[row] = []
         self.table[row].zero_()
+
+
+class Paged8KVCache(PagedKVCache):
+    """The same pages held in 8 bits: per layer K and V codes uint8 [num_pages,
+    Hkv, page_size, D] (code + 128) and scales fp32 [num_pages, Hkv, page_size /
+    16], one for 16 consecutive positions of a head -- half the memory and half
+    the bytes a decode step reads (``ops.functional.rope_kv8_append``,
+    ``kv8_decode_attention``, ``gather_kv8``). A block's scale starts anew with
+    its first position, so a released page needs no clearing."""
+
+    def _make_pools(self, n_layers: int, num_pages: int, n_kv_heads: int, head_dim: int, device) -> None:
+        if self.page_size < 16 or head_dim not in (64, 128):
+            raise ValueError("8-bit KV cache: pages of at least 16 tokens, head_dim 64 or 128")
+        shape = (num_pages, n_kv_heads, self.page_size, head_dim)
+        self.k, self.v = ([torch.full(shape, 128, dtype=torch.uint8, device=device) for _ in range(n_layers)]
+                          for _ in range(2))
+        scales = (num_pages, n_kv_heads, self.page_size // 16)
+        self.ks, self.vs = ([torch.zeros(scales, device=device) for _ in range(n_layers)] for _ in range(2))
+
+    def bytes(self) -> int:
+        return sum(t.numel() for t in self.k + self.v) + sum(t.numel() * 4 for t in self.ks + self.vs)
+
+    def layer(self, i: int) -> tuple:
+        """(K codes, K scales, V codes, V scales) of layer i."""
+        return self.k[i], self.ks[i], self.v[i], self.vs[i]

@@ -247,6 +247,11 @@ def main():
     ap.add_argument("--keep-quant", action="store_true",
                     help="with --gguf: keep the projections in the file's quantised blocks on the device (the "
                     "file's size in memory) and expand each right before its GEMM")
+    ap.add_argument("--w4", type=int, default=0, metavar="GROUP",
+                    help="quantise the projections to 4 bits with a scale for each GROUP columns (32, 64 or 128; dense "
+                         "models, one GPU)")
+    ap.add_argument("--kv-bits", type=int, default=16, choices=[8, 16],
+                    help="8: paged KV cache in 8 bits (dense models)")
     ap.add_argument("--hf", default=None, help="load Qwen2 weights from a Hugging Face directory")
     ap.add_argument("--tp", type=int, default=1,
                     help="tensor-parallel degree; launch with torchrun --nproc-per-node N (rank 0 serves HTTP)")
@@ -322,8 +327,13 @@ def main():
     elif isinstance(cfg, MoEConfig):
         model = MoEQwenModel(cfg, device=args.device, max_batch=args.max_concurrent, max_seq=args.max_seq, tp=tp)
     else:
+        if args.w4:
+            if args.tp > 1:
+                raise SystemExit("--w4 serves one GPU (the TP shards are bf16)")
+            weights = (weights or QwenWeights(cfg, args.device)).quantize_w4(args.w4)
+        pages = args.max_concurrent * -(-args.max_seq // 64) + 1 if args.kv_bits == 8 else 0
         model = QwenModel(cfg, device=args.device, max_batch=args.max_concurrent, max_seq=args.max_seq,
-                          weights=weights, tp=tp)
+                          weights=weights, tp=tp, kv_pages=pages, kv_bits=args.kv_bits)
     if tp is not None:
         if info.rank != 0:
             follow(model, ctrl)  # until rank 0 stops
