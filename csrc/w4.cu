@@ -2,50 +2,17 @@
 //
 //   y[m, n] = sum_g s[n, g] * sum_{k in group g} (c[n, k] - 8) * x[m, k]
 //
-// Weights [N, K] are laid out once for the kernel that streams them: int32
-// q [ceil(N/16), ceil(K/128), 2, 32, 4] and fp16 scales
-// [ceil(N/16), ceil(K/128) * 128 / group, 8, 2]. Tile (n, k) holds rows 16 n ..
-// and columns 128 k ..; [h, l, j] of it is row 8 h + l / 4, and element e of
-// its eight is column 16 (2 j + e / 4) + 4 (l % 4) + e % 4, in bits
-// {0, 16, 4, 20, 8, 24, 12, 28}[e]. scales[n, g, r, h] belongs to row 8 h + r.
-// Rows and columns past N and K are padding (code 8, scale 0).
+// (layout in w4.cuh)
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
-#include <cuda_fp16.h>
 
 #include "common.cuh"
 #include "host_utils.h"
+#include "w4.cuh"
 
 namespace aether {
 namespace w4 {
-
-struct Weight {
-  const uint32_t* q;
-  const __half* s;
-  int N, K, kt, groups, gshift;  // kt: column tiles; groups: scales of a row; gshift: log2(group)
-};
-
-__device__ __forceinline__ float scale_at(const Weight& w, int n, int k) {
-  return __half2float(w.s[(((int64_t)(n >> 4) * w.groups + (k >> w.gshift)) * 8 + (n & 7)) * 2 + ((n >> 3) & 1)]);
-}
-__device__ __forceinline__ int code_at(uint32_t word, int e) {
-  return (int)((word >> (4 * (e >> 1) + 16 * (e & 1))) & 15u) - 8;
-}
-
-struct LinearParams {
-  Weight w;
-  const __nv_bfloat16* x;
-  int64_t xs;
-  const __nv_bfloat16* bias;
-  const __nv_bfloat16* res;
-  int64_t rs;
-  __nv_bfloat16* y;
-  int64_t ys;
-  int M, n_out, swiglu;
-  int outs, tiles, S, per;  // outputs of a CTA and how many such; parts of the columns and their column tiles
-  int* status;
-};
 
 // A CTA's eight multiplying warps own 128 / KH rows, a tile of 16 each (SwiGLU:
 // gate tiles and the up tiles they meet), and, in a cluster of S, the S-th part
@@ -69,55 +36,9 @@ constexpr int kThreads = kWarps * 32 + 32;
 constexpr int kPair = 2;                    // column tiles of a ring stage
 constexpr int kRing = 4;                    // stages of a warp's ring
 
-// A constant that stays in a register: written as an immediate, it is moved into one again for each use.
-__device__ __forceinline__ uint32_t in_register(uint32_t c) {
-  uint32_t r;
-  asm volatile("mov.u32 %0, %1;" : "=r"(r) : "r"(c));
-  return r;
-}
-struct Consts {
-  uint32_t mask, bias, minus;  // 0x000f000f, 0x43004300 (128), 0xc308c308 (-136)
-};
-// bf16 pair of two weight codes (nibbles i and i + 4 of w), exact
-template <int i>
-__device__ __forceinline__ uint32_t codes2(uint32_t w, const Consts& k) {
-  uint32_t x, r;
-  asm("lop3.b32 %0, %1, %2, %3, 0xea;" : "=r"(x) : "r"(w >> (4 * i)), "r"(k.mask), "r"(k.bias));  // (a & b) | c
-  asm("add.rn.bf16x2 %0, %1, %2;" : "=r"(r) : "r"(x), "r"(k.minus));
-  return r;
-}
-__device__ __forceinline__ void mma_bf16(float (&c)[4], const uint32_t (&a)[4], uint32_t b0, uint32_t b1) {
-  asm volatile(
-      "mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, {%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
-      : "+f"(c[0]), "+f"(c[1]), "+f"(c[2]), "+f"(c[3])
-      : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
-}
-__device__ __forceinline__ float4 ld_cluster4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared::cluster.v4.f32 {%0,%1,%2,%3}, [%4];"
-               : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint4 lds128(uint32_t addr) {
-  uint4 v;
-  asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ uint32_t lds32(uint32_t addr) {
-  uint32_t v;
-  asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
-  return v;
-}
-__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src) {
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
-}
-__device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, bool in) {  // zeros where not `in`
-  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
-}
-
 // MT: tiles of eight token rows; GS: k16 steps of a scale group (2, 4 or 8); KH: parts of the columns side by side
 template <int MT, int GS, int KH>
-__global__ void __launch_bounds__(kThreads, MT <= 2 ? 2 : 1) linear_kernel(LinearParams p) {
+__global__ void __launch_bounds__(kThreads, 2) linear_kernel(LinearParams p) {
   constexpr int kGroups = 8 / GS;  // of a column tile
   constexpr int kRowTiles = kWarps / KH;
   constexpr int kTileBytes = 1024 + kGroups * 32;
@@ -278,54 +199,7 @@ __global__ void __launch_bounds__(kThreads, MT <= 2 ? 2 : 1) linear_kernel(Linea
       }
   }
   if (S > 1) cluster_sync(); else __syncthreads();
-  const uint32_t own = smem_u32(smem);
-  constexpr int kUpAt = kRowTiles * 8;  // SwiGLU: the first up tile's place among the rows
-  auto sum_at = [&](int tok, int row) {  // four rows, all parts of all ranks
-    float4 v[8], w = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int h = 0; h < KH; ++h) {
-      const uint32_t a = own + ((h * p.M + tok) * kLd + row) * 4;
-#pragma unroll
-      for (int c = 0; c < 8; ++c) {
-        v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < S) v[c] = ld_cluster4(S > 1 ? mapa_shared(a, c) : a);
-      }
-#pragma unroll
-      for (int c = 0; c < 8; ++c) w.x += v[c].x, w.y += v[c].y, w.z += v[c].z, w.w += v[c].w;
-    }
-    return w;
-  };
-  const int quads = p.M * p.outs / 4, share = (quads + S - 1) / S;
-  for (int e = rank * share + tid; e < min(quads, (rank + 1) * share); e += kThreads) {
-    const int tok = e / (p.outs / 4), i = e % (p.outs / 4) * 4;
-    if (n0 + i >= p.n_out) continue;
-    const float4 v4 = sum_at(tok, i);
-    float v[4] = {v4.x, v4.y, v4.z, v4.w};
-    float u[4] = {0.f, 0.f, 0.f, 0.f};
-    if (p.swiglu) {  // up rows start `up` rows into their tiles: from the two aligned quads around them
-      const int o = up & 3;
-      const float4 a = sum_at(tok, kUpAt + ((up + i) & ~3));
-      float4 c = a;
-      if (o) c = sum_at(tok, kUpAt + ((up + i) & ~3) + 4);
-      u[0] = o == 0 ? a.x : o == 1 ? a.y : o == 2 ? a.z : a.w;
-      u[1] = o == 0 ? a.y : o == 1 ? a.z : o == 2 ? a.w : c.x;
-      u[2] = o == 0 ? a.z : o == 1 ? a.w : o == 2 ? c.x : c.y;
-      u[3] = o == 0 ? a.w : o == 1 ? c.x : o == 2 ? c.y : c.z;
-    }
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-      const int n = n0 + i + k;
-      if (n < p.n_out) {
-        if (p.bias) v[k] += __bfloat162float(p.bias[n]);
-        if (p.swiglu) {
-          if (p.bias) u[k] += __bfloat162float(p.bias[p.n_out + n]);
-          v[k] = v[k] / (1.f + __expf(-v[k])) * u[k];
-        }
-        if (p.res) v[k] += __bfloat162float(p.res[tok * p.rs + n]);
-        p.y[tok * p.ys + n] = __float2bfloat16(v[k]);
-      }
-    }
-  }
+  finish<KH, kLd, kRowTiles * 8>(p, smem_u32(smem), S, rank, n0, up, tid, kThreads);
   if (S > 1) cluster_sync();  // every CTA's sums are read before its shared memory goes
 }
 
@@ -359,11 +233,11 @@ static void launch_linear(LinearParams& p, cudaStream_t st) {
 }
 // Rows of a CTA and parts of the columns. An SM's fullest load is n CTAs of (column tiles + 4 for their start and end)
 // each; one alone leaves issue slots empty, two hide each other's waits.
-static int plan(LinearParams& p, int most_parts) {
+static int plan(LinearParams& p) {
   const int sms = num_sms(current_device());
   float best = 0.f;
   int kh = 1;
-  for (int h = 1; h <= most_parts; ++h) {
+  for (int h = 1; h <= 2; ++h) {
     const int rows = 128 / h;
     const int outs = !p.swiglu ? rows : p.n_out % 16 == 0 ? rows / 2 : rows / 2 - 16;  // (see row_tile: one tile more)
     const int tiles = (p.n_out + outs - 1) / outs;
@@ -378,15 +252,10 @@ static int plan(LinearParams& p, int most_parts) {
 }
 template <int MT, int GS>
 static void launch_parts(LinearParams& p, cudaStream_t st) {
-  if constexpr (MT == 8) {  // two parts' token rows would not fit beside three stages
-    plan(p, 1);
+  if (plan(p) == 1)
     launch_linear<MT, GS, 1>(p, st);
-  } else {
-    if (plan(p, 2) == 1)
-      launch_linear<MT, GS, 1>(p, st);
-    else
-      launch_linear<MT, GS, 2>(p, st);
-  }
+  else
+    launch_linear<MT, GS, 2>(p, st);
 }
 template <int MT>
 static void launch_group(LinearParams& p, cudaStream_t st) {
@@ -493,10 +362,8 @@ at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_
     launch_group<1>(p, st);
   else if (M <= 16)
     launch_group<2>(p, st);
-  else if (M <= 32)
-    launch_group<4>(p, st);
   else
-    launch_group<8>(p, st);
+    linear_w4_tc(p, st);
   return y;
 }
 

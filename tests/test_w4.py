@@ -63,6 +63,27 @@ def test_linear_columns_that_end_inside_a_tile(dev, K, group):
 
 
 @pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("M", [16, 17, 32, 33, 48, 64])
+@pytest.mark.parametrize("N,K,group", [(35, 32, 32), (130, 96, 32), (300, 192, 64), (515, 1920, 128), (1000, 1056, 32)])
+def test_linear_batches(dev, M, N, K, group):
+    check(dev, M, N, K, group, bias=True, residual=True, wide=5)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
+@pytest.mark.parametrize("M,F_", [(17, 200), (40, 64), (64, 1000), (64, 33)])
+def test_linear_batches_swiglu(dev, M, F_):
+    check(dev, M, 2 * F_, 512, 64, bias=True, swiglu=True)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("group", [32, 64, 128])
+def test_gpu_linear_more_row_tiles_than_sms(group):
+    """A CTA walks over several row tiles, its pipelines running on."""
+    check("cuda", 64, 128 * 330 + 7, 384, group)
+    check("cuda", 20, 128 * 330 + 7, 384, group, bias=True)
+
+
+@pytest.mark.parametrize("dev", CPU_GPU)
 @pytest.mark.parametrize("M,N,K,bias,residual,swiglu", [(1, 200, 256, True, True, False), (4, 2 * 133, 512, False, False, True),
                                                         (16, 2 * 64, 384, True, False, True), (33, 130, 640, True, True, False),
                                                         (2, 6, 128, True, True, True)])
