@@ -81,15 +81,18 @@ __device__ __forceinline__ bool mbar_try_wait(uint32_t addr, uint32_t parity) {
 
 // Bounded wait on an mbarrier phase. Returns false if the wait gave up, either
 // because the time limit passed or because another role raised `abort_word`.
+// The clock is read only once a wait has failed 64 times: reading it takes about
+// a microsecond, which every short wait of a pipeline would pay.
 __device__ __forceinline__ bool mbar_wait(uint64_t* bar, uint32_t parity, volatile int* abort_word) {
   const uint32_t addr = smem_u32(bar);
-  if (mbar_try_wait(addr, parity)) return true;
-  const uint64_t t0 = globaltimer_ns();
+  uint64_t t0 = 0;
   for (uint32_t it = 1;; ++it) {
     if (mbar_try_wait(addr, parity)) return true;
     if ((it & 63u) == 0u) {
       if (*abort_word) return false;
-      if (globaltimer_ns() - t0 > kWaitTimeoutNs) return false;
+      const uint64_t now = globaltimer_ns();
+      if (t0 == 0) t0 = now;
+      if (now - t0 > kWaitTimeoutNs) return false;
     }
   }
 }

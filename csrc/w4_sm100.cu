@@ -5,7 +5,7 @@
 //
 // A CTA owns 128 weight rows -- the 128 lanes of TMEM -- and, in a cluster of S,
 // the S-th part of the columns. Eight warps unpack: each streams the codes of 16
-// rows through its own ring (16-byte asynchronous copies, 13 column tiles ahead)
+// rows through its own ring (16-byte asynchronous copies, 12 column tiles ahead)
 // and writes exact bf16 codes straight into TMEM, where a lane's registers are
 // already in the order that a 16 x 256-bit store wants, so the unpacked weights
 // never pass through shared memory. One thread issues tcgen05.mma with the codes
@@ -30,14 +30,15 @@ namespace tc {
 constexpr int kUnpack = 8;                   // warps that unpack, one row tile each
 constexpr int kScale = 4;                    // warps that scale, 32 rows each
 constexpr int kLoader = kUnpack + kScale;    // warp of the token rows
-constexpr int kIssuer = kLoader + 1;         // warp of the tensor cores
-constexpr int kThreads = (kIssuer + 1) * 32;
-constexpr int kRing = 14;                    // column tiles of a warp's ring
-constexpr int kA = 3;                        // column tiles of unpacked codes in TMEM, 64 columns each
+constexpr int kIssuer = kLoader + 1;         // first warp of the tensor cores
+constexpr int kIssuers = 2;                  // take column tiles in turn: one spends as long on its waits as on its products
+constexpr int kThreads = (kIssuer + kIssuers) * 32;
+constexpr int kRing = 13;                    // column tiles of an unpacking warp's ring
+constexpr int kStages = 4;                   // column tiles of codes in TMEM (64 columns each) and of token rows
 constexpr int kD = 4;                        // accumulators in TMEM, 64 columns each
-constexpr int kX = 4;                        // column tiles of token rows in shared memory
+constexpr int kFar = 12;                     // column tiles of scales of a scaling warp's ring
 constexpr int kLd = 128 + 4;                 // floats of one token's sums
-constexpr int kColsA = kD * 64;              // first TMEM column of the codes
+constexpr int kColsA = kD * 64;              // first TMEM column of the codes (all 512 are in use)
 
 // 16 lanes x 64 columns: a thread's registers 4 i .. are (lane l / 4, columns 8 i + 2 (l % 4) and the next), then lane
 // l / 4 + 8
@@ -66,22 +67,27 @@ struct Pipe {  // place and phase in a ring of N
 template <int NP, int GS>
 __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_constant__ CUtensorMap xmap, LinearParams p) {
   constexpr int kGroups = 8 / GS;  // of a column tile
+  // The issuers take turns by groups where a column tile's groups use every accumulator, else by column tiles: each
+  // always meets the same accumulators and stages, so that no phase of theirs passes it by.
+  constexpr bool kByGroup = kGroups == kD;
+  static_assert(kStages % kIssuers == 0 && kD % kIssuers == 0 && (kByGroup || kD % (kGroups * kIssuers) == 0), "turns");
   constexpr int kXBytes = 2 * NP * 128;
   extern __shared__ __align__(1024) uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
-  uint8_t* s_x = smem;                                  // [kX][2][NP][128 bytes]
-  uint8_t* s_ring = s_x + kX * kXBytes;                 // [kUnpack][kRing][1024]
-  float* s_sums = reinterpret_cast<float*>(s_ring + kUnpack * kRing * 1024);  // [M][kLd]
-  __shared__ __align__(8) uint64_t a_full[kA], a_empty[kA], x_full[kX], x_empty[kX], d_full[kD], d_empty[kD], drain;
+  uint8_t* s_x = smem;                                        // [kStages][2][NP][128 bytes]
+  uint8_t* s_ring = s_x + kStages * kXBytes;                  // [kUnpack][kRing][1024]
+  uint8_t* s_scales = s_ring + kUnpack * kRing * 1024;        // [kScale][kFar][2 row tiles][kGroups][32 bytes]
+  float* s_sums = reinterpret_cast<float*>(s_scales + kScale * kFar * kGroups * 64);  // [M][kLd]
+  // full: a column tile's codes are in TMEM and its token rows in shared memory; free: its products are done
+  __shared__ __align__(8) uint64_t full[kStages], free_[kStages], d_full[kD], d_empty[kD], drain[kIssuers];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   if (tid == 0) {
     s_abort = 0;
-    for (int i = 0; i < kA; ++i) mbar_init(a_full + i, kUnpack), mbar_init(a_empty + i, 1);
-    for (int i = 0; i < kX; ++i) mbar_init(x_full + i, 1), mbar_init(x_empty + i, 1);
+    for (int i = 0; i < kStages; ++i) mbar_init(full + i, kUnpack + 1), mbar_init(free_ + i, kByGroup ? kIssuers : 1);
     for (int i = 0; i < kD; ++i) mbar_init(d_full + i, 1), mbar_init(d_empty + i, kScale);
-    mbar_init(&drain, 1);
+    for (int i = 0; i < kIssuers; ++i) mbar_init(drain + i, 1);
     fence_mbar_init();
     fence_async_smem();
   }
@@ -154,59 +160,71 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
           out[4 * s + 6] = codes2<2>(wb[s >> 1], k);
           out[4 * s + 7] = codes2<3>(wb[s >> 1], k);
         }
-        if (!wait(a_empty + a.at, a.phase ^ 1)) break;
+        if (!wait(free_ + a.at, a.phase ^ 1)) break;
         __syncwarp();
         tc_fence_after();
         tmem_st_16x256b_x8(to + a.at * 64, out);
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
-        if (lane == 0) mbar_arrive(a_full + a.at);
-        a.next<kA>();
+        if (lane == 0) mbar_arrive(full + a.at);
+        a.next<kStages>();
       }
     asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp < kLoader) {
     // ------------------------------------------------------------ scales and sums
-    const int quad = warp & 3, row = quad * 32 + lane, rt = row >> 4;
+    const int quad = warp & 3, row = quad * 32 + lane;
     const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16);
-    constexpr int kFar = GS == 2 ? 2 : 4;  // column tiles that scales are loaded ahead
+    // the scales of the warp's two row tiles: 64 bytes a group, 16 to a lane
+    constexpr int kBytes = kGroups * 64;
+    const uint32_t ring = smem_u32(s_scales) + (warp - kUnpack) * (kFar * kBytes);
+    int f_tile = tile0, f_i = 0, f_at = 0;
+    const uint8_t* sc = nullptr;
+    auto fetch = [&]() {
+      if (f_tile < p.tiles && n_kt > 0) {
+        if (f_i == 0)
+          sc = reinterpret_cast<const uint8_t*>(p.w.s) +
+               ((int64_t)row_tile(f_tile, 2 * quad + lane / (2 * kGroups) % 2) * p.w.groups + (int64_t)c0 * kGroups) * 32 +
+               lane % (2 * kGroups) * 16;
+        if (lane < 4 * kGroups) cp_async16(ring + f_at * kBytes + lane * 16, sc);
+        sc += kGroups * 32;
+        if (++f_i == n_kt) f_i = 0, f_tile += tile_step;
+      }
+      asm volatile("cp.async.commit_group;" ::: "memory");
+      if (++f_at == kFar) f_at = 0;
+    };
+    for (int i = 0; i < kFar - 1; ++i) fetch();
+    const uint32_t mine = ring + (lane >> 4) * (kGroups * 32) + (row & 7) * 4 + ((row >> 3) & 1) * 2;
+    int at = 0;
     Pipe d;
     for (int tile = tile0; tile < p.tiles; tile += tile_step) {  // (all of them: the four warps meet at a barrier)
-      const __half* sc = p.w.s + ((int64_t)row_tile(tile, rt) * p.w.groups + (int64_t)c0 * kGroups) * 16 + (row & 7) * 2 + ((row >> 3) & 1);
-      __half far[kFar][kGroups];
-#pragma unroll
-      for (int u = 0; u < kFar; ++u)
-#pragma unroll
-        for (int g = 0; g < kGroups; ++g) far[u][g] = u < n_kt ? sc[(u * kGroups + g) * 16] : __half();
       float acc[NP];
 #pragma unroll
       for (int n = 0; n < NP; ++n) acc[n] = 0.f;
-      for (int i = 0; i < n_kt; i += kFar) {
+      for (int i = 0; i < n_kt; ++i) {
+        asm volatile("cp.async.wait_group %0;" ::"n"(kFar - 2) : "memory");
+        __syncwarp();
+        fetch();
 #pragma unroll
-        for (int u = 0; u < kFar; ++u) {
-          if (i + u < n_kt) {
+        for (int g = 0; g < kGroups; ++g) {
+          uint16_t h;
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(mine + at * kBytes + g * 32) : "memory");
+          const float s = __half2float(__ushort_as_half(h));
+          wait(d_full + d.at, d.phase);
+          __syncwarp();
+          tc_fence_after();
+          uint32_t v[NP];
 #pragma unroll
-            for (int g = 0; g < kGroups; ++g) {
-              const float s = __half2float(far[u][g]);
-              if (i + u + kFar < n_kt) far[u][g] = sc[((i + u + kFar) * kGroups + g) * 16];
-              wait(d_full + d.at, d.phase);
-              __syncwarp();
-              tc_fence_after();
+          for (int c = 0; c < NP; c += 32) tmem_ld32(from + d.at * 64 + c, *reinterpret_cast<uint32_t(*)[32]>(v + c));
+          tmem_ld_wait();
+          tc_fence_before();
+          __syncwarp();
+          if (lane == 0) mbar_arrive(d_empty + d.at);
 #pragma unroll
-              for (int c = 0; c < NP; c += 32) {
-                uint32_t v[32];
-                tmem_ld32(from + d.at * 64 + c, v);
-                tmem_ld_wait();
-#pragma unroll
-                for (int n = 0; n < 32; ++n) acc[c + n] += s * __uint_as_float(v[n]);
-              }
-              tc_fence_before();
-              __syncwarp();
-              if (lane == 0) mbar_arrive(d_empty + d.at);
-              d.next<kD>();
-            }
-          }
+          for (int n = 0; n < NP; ++n) acc[n] += s * __uint_as_float(v[n]);
+          d.next<kD>();
         }
+        if (++at == kFar) at = 0;
       }
 #pragma unroll
       for (int n = 0; n < NP; ++n)
@@ -218,46 +236,57 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
         asm volatile("bar.sync 1, 128;" ::: "memory");  // the sums are free again
       }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kLoader) {
     // ------------------------------------------------------------ token rows
     if (lane == 0) {
       Pipe x;
       for (int tile = tile0; tile < p.tiles && ok; tile += tile_step)
         for (int i = 0; i < n_kt; ++i) {
-          if (!wait(x_empty + x.at, x.phase ^ 1)) break;
-          mbar_arrive_expect_tx(x_full + x.at, kXBytes);
-          tma_load_2d(s_x + x.at * kXBytes, &xmap, x_full + x.at, (c0 + i) * 128, 0);
-          tma_load_2d(s_x + x.at * kXBytes + kXBytes / 2, &xmap, x_full + x.at, (c0 + i) * 128 + 64, 0);
-          x.next<kX>();
+          if (!wait(free_ + x.at, x.phase ^ 1)) break;
+          mbar_arrive_expect_tx(full + x.at, kXBytes);
+          tma_load_2d(s_x + x.at * kXBytes, &xmap, full + x.at, (c0 + i) * 128, 0);
+          tma_load_2d(s_x + x.at * kXBytes + kXBytes / 2, &xmap, full + x.at, (c0 + i) * 128 + 64, 0);
+          x.next<kStages>();
         }
     }
   } else if (lane == 0) {
     // ------------------------------------------------------------ tensor cores
     constexpr uint32_t idesc = idesc_bf16_f32(128, NP, false, false);
-    Pipe a, x, d;
+    const int who = warp - kIssuer;
+    Pipe a, d;
+    int turn = 0;
     for (int tile = tile0; tile < p.tiles && ok; tile += tile_step)
       for (int i = 0; i < n_kt && ok; ++i) {
-        if (!wait(x_full + x.at, x.phase) || !wait(a_full + a.at, a.phase)) break;
-        const uint32_t b = smem_u32(s_x + x.at * kXBytes), codes = tmem + kColsA + a.at * 64;
+        if (kByGroup || turn == who) {
+          if (!wait(full + a.at, a.phase)) break;
+          const uint32_t b = smem_u32(s_x + a.at * kXBytes), codes = tmem + kColsA + a.at * 64;
 #pragma unroll
-        for (int g = 0; g < kGroups; ++g) {
-          if (!wait(d_empty + d.at, d.phase ^ 1)) break;
-          tc_fence_after();
+          for (int g = 0; g < kGroups; ++g) {
+            if (kByGroup && g % kIssuers != who) {
+              d.next<kD>();
+              continue;
+            }
+            if (!wait(d_empty + d.at, d.phase ^ 1)) break;
+            tc_fence_after();
 #pragma unroll
-          for (int s = g * GS; s < (g + 1) * GS; ++s)
-            umma_f16_ts(tmem + d.at * 64, codes + s * 8, sdesc_sw128(b + (s >> 2) * (kXBytes / 2) + (s & 3) * 32, 16, 1024), idesc,
-                        s != g * GS ? 1u : 0u);
-          umma_commit(d_full + d.at);
-          d.next<kD>();
+            for (int s = g * GS; s < (g + 1) * GS; ++s)
+              umma_f16_ts(tmem + d.at * 64, codes + s * 8, sdesc_sw128(b + (s >> 2) * (kXBytes / 2) + (s & 3) * 32, 16, 1024),
+                          idesc, s != g * GS ? 1u : 0u);
+            umma_commit(d_full + d.at);
+            d.next<kD>();
+          }
+          umma_commit(free_ + a.at);
+        } else {
+#pragma unroll
+          for (int g = 0; g < kGroups; ++g) d.next<kD>();
         }
-        umma_commit(a_empty + a.at);
-        umma_commit(x_empty + x.at);
-        a.next<kA>();
-        x.next<kX>();
+        a.next<kStages>();
+        if (++turn == kIssuers) turn = 0;
       }
     volatile int never = 0;
-    umma_commit(&drain);
-    mbar_wait(&drain, 0, &never);
+    umma_commit(drain + who);
+    mbar_wait(drain + who, 0, &never);
   }
   if (!ok) atomicExch(p.status, kStatusTimeoutMma);
   __syncwarp();
@@ -280,7 +309,7 @@ static void launch(LinearParams& p, cudaStream_t st) {
   // SwiGLU: four gate tiles meet four up tiles, or three gate tiles four, where the up rows start inside a tile
   p.outs = !p.swiglu ? 128 : p.n_out % 16 == 0 ? 64 : 48;
   p.tiles = (p.n_out + p.outs - 1) / p.outs;
-  constexpr int kFixed = kX * 2 * NP * 128 + kUnpack * kRing * 1024 + 1024;
+  constexpr int kFixed = kStages * 2 * NP * 128 + kUnpack * kRing * 1024 + kScale * kFar * (8 / GS) * 64 + 1024;
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
