@@ -78,6 +78,11 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
+__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
+  float4 v;
+  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
+  return v;
+}
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -102,20 +107,32 @@ __device__ __forceinline__ void finish(const LinearParams& p, uint32_t own, int 
 #pragma unroll
     for (int h = 0; h < KH; ++h) {
       const uint32_t a = own + ((h * p.M + tok) * kLd + row) * 4;
+      if (S == 1) {
+        v[0] = lds_f4(a);
+        w.x += v[0].x, w.y += v[0].y, w.z += v[0].z, w.w += v[0].w;
+        continue;
+      }
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < S) v[c] = ld_cluster4(S > 1 ? mapa_shared(a, c) : a);
+        if (c < S) v[c] = ld_cluster4(mapa_shared(a, c));
       }
 #pragma unroll
       for (int c = 0; c < 8; ++c) w.x += v[c].x, w.y += v[c].y, w.z += v[c].z, w.w += v[c].w;
     }
     return w;
   };
-  const int quads = p.M * p.outs / 4, share = (quads + S - 1) / S;
-  for (int e = rank * share + tid; e < min(quads, (rank + 1) * share); e += nthreads) {
-    const int tok = e / (p.outs / 4), i = e % (p.outs / 4) * 4;
-    if (n0 + i >= p.n_out) continue;
+  // outputs and residuals as 8 bytes of four where their rows allow it
+  const bool wide = p.ys % 4 == 0 && reinterpret_cast<uintptr_t>(p.y) % 8 == 0 &&
+                    (p.res == nullptr || (p.rs % 4 == 0 && reinterpret_cast<uintptr_t>(p.res) % 8 == 0));
+  const int per = p.outs / 4, quads = p.M * per, share = (quads + S - 1) / S;
+  const int end = min(quads, (rank + 1) * share);
+  int e = rank * share + tid, tok = e / per, q = e - tok * per;
+  const int step_tok = nthreads / per, step_q = nthreads - step_tok * per;
+  for (; e < end; e += nthreads, tok += step_tok, q += step_q) {
+    if (q >= per) q -= per, ++tok;
+    const int i = q * 4, n = n0 + i;
+    if (n >= p.n_out) continue;
     const float4 v4 = sum_at(tok, i);
     float v[4] = {v4.x, v4.y, v4.z, v4.w};
     float u[4] = {0.f, 0.f, 0.f, 0.f};
@@ -129,19 +146,25 @@ __device__ __forceinline__ void finish(const LinearParams& p, uint32_t own, int 
       u[2] = o == 0 ? a.z : o == 1 ? a.w : o == 2 ? c.x : c.y;
       u[3] = o == 0 ? a.w : o == 1 ? c.x : o == 2 ? c.y : c.z;
     }
+    const bool whole = wide && n + 4 <= p.n_out;
+    float r[4] = {0.f, 0.f, 0.f, 0.f};
+    if (p.res && whole) {
+      const uint2 w = *reinterpret_cast<const uint2*>(p.res + tok * p.rs + n);
+      r[0] = bf16lo(w.x), r[1] = bf16hi(w.x), r[2] = bf16lo(w.y), r[3] = bf16hi(w.y);
+    }
 #pragma unroll
     for (int k = 0; k < 4; ++k) {
-      const int n = n0 + i + k;
-      if (n < p.n_out) {
-        if (p.bias) v[k] += __bfloat162float(p.bias[n]);
-        if (p.swiglu) {
-          if (p.bias) u[k] += __bfloat162float(p.bias[p.n_out + n]);
-          v[k] = v[k] / (1.f + __expf(-v[k])) * u[k];
-        }
-        if (p.res) v[k] += __bfloat162float(p.res[tok * p.rs + n]);
-        p.y[tok * p.ys + n] = __float2bfloat16(v[k]);
+      if (n + k >= p.n_out) break;
+      if (p.bias) v[k] += __bfloat162float(p.bias[n + k]);
+      if (p.swiglu) {
+        if (p.bias) u[k] += __bfloat162float(p.bias[p.n_out + n + k]);
+        v[k] = __fdividef(v[k], 1.f + __expf(-v[k])) * u[k];
       }
+      if (p.res && !whole) r[k] = __bfloat162float(p.res[tok * p.rs + n + k]);
+      v[k] += r[k];
+      if (!whole) p.y[tok * p.ys + n + k] = __float2bfloat16(v[k]);
     }
+    if (whole) *reinterpret_cast<uint2*>(p.y + tok * p.ys + n) = make_uint2(pack_bf16(v[0], v[1]), pack_bf16(v[2], v[3]));
   }
 }
 
