@@ -29,7 +29,9 @@ _KERNELS_PER_CALL = {
 
 
 class _CountingModule:
-    """Proxy over ``_C`` that counts kernel launches while counting is on."""
+    """Proxy over ``_C`` that counts kernel launches while counting is on.
+    Functions are kept as attributes once looked up: bare while counting is
+    off, wrapped while it is on."""
 
     def __init__(self, mod):
         self._mod = mod
@@ -40,15 +42,19 @@ class _CountingModule:
         fn = getattr(self._mod, name)
         if not callable(fn):
             return fn
-        k = _KERNELS_PER_CALL.get(name, 1)
+        if self.enabled:
+            bare, k = fn, _KERNELS_PER_CALL.get(name, 1)
 
-        def wrapped(*a, _fn=fn, _k=k, **kw):
-            if self.enabled:
-                self.launches += _k
-            return _fn(*a, **kw)
+            def fn(*a, **kw):
+                self.launches += k
+                return bare(*a, **kw)
 
-        setattr(self, name, wrapped)  # found without this method from now on
-        return wrapped
+        setattr(self, name, fn)  # found without this method from now on
+        return fn
+
+    def count(self, enable: bool) -> None:
+        if enable != self.enabled:
+            self.__dict__ = {"_mod": self._mod, "enabled": enable, "launches": self.launches}
 
 
 _PROXY = _CountingModule(_C) if _C is not None else None
@@ -61,7 +67,7 @@ def count_launches(enable: bool) -> int:
     n = _PROXY.launches
     if enable:
         _PROXY.launches = 0
-    _PROXY.enabled = enable
+    _PROXY.count(enable)
     return n
 
 

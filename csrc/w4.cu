@@ -199,7 +199,7 @@ __global__ void __launch_bounds__(kThreads, 2) linear_kernel(LinearParams p) {
       }
   }
   if (S > 1) cluster_sync(); else __syncthreads();
-  finish<KH, kLd, kRowTiles * 8>(p, smem_u32(smem), S, rank, n0, up, tid, kThreads);
+  finish<KH, kLd, kRowTiles * 8>(p, reinterpret_cast<const float*>(smem), S, rank, n0, up, tid, kThreads);
   if (S > 1) cluster_sync();  // every CTA's sums are read before its shared memory goes
 }
 

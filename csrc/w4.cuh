@@ -78,11 +78,6 @@ __device__ __forceinline__ uint4 lds128(uint32_t addr) {
   asm volatile("ld.shared.v4.u32 {%0,%1,%2,%3}, [%4];" : "=r"(v.x), "=r"(v.y), "=r"(v.z), "=r"(v.w) : "r"(addr) : "memory");
   return v;
 }
-__device__ __forceinline__ float4 lds_f4(uint32_t addr) {
-  float4 v;
-  asm volatile("ld.shared.v4.f32 {%0,%1,%2,%3}, [%4];" : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
-  return v;
-}
 __device__ __forceinline__ uint32_t lds32(uint32_t addr) {
   uint32_t v;
   asm volatile("ld.shared.u32 %0, [%1];" : "=r"(v) : "r"(addr) : "memory");
@@ -95,27 +90,28 @@ __device__ __forceinline__ void cp_async16_zfill(uint32_t dst, const void* src, 
   asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(in ? 16 : 0) : "memory");
 }
 
-// A CTA's share of a cluster's outputs, four rows to a thread: the sums
-// [part][token][kLd] at shared address `own` of each of the S CTAs, in the order
+// A CTA's share of a cluster's outputs, four rows to a thread: `sums`
+// [part][token][kLd] in the shared memory of each of the S CTAs, in the order
 // of the columns, then bias, SwiGLU (up rows `up` rows into their tiles, which
 // start at kUpAt) and residual.
 template <int KH, int kLd, int kUpAt>
-__device__ __forceinline__ void finish(const LinearParams& p, uint32_t own, int S, int rank, int n0, int up, int tid,
-                                       int nthreads) {
+__device__ __forceinline__ void finish(const LinearParams& p, const float* sums, int S, int rank, int n0, int up,
+                                       int tid, int nthreads) {
+  const uint32_t own = smem_u32(sums);
   auto sum_at = [&](int tok, int row) {  // four rows, all parts of all ranks
     float4 v[8], w = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int h = 0; h < KH; ++h) {
-      const uint32_t a = own + ((h * p.M + tok) * kLd + row) * 4;
+      const int at = (h * p.M + tok) * kLd + row;
       if (S == 1) {
-        v[0] = lds_f4(a);
+        v[0] = *reinterpret_cast<const float4*>(sums + at);
         w.x += v[0].x, w.y += v[0].y, w.z += v[0].z, w.w += v[0].w;
         continue;
       }
 #pragma unroll
       for (int c = 0; c < 8; ++c) {
         v[c] = make_float4(0.f, 0.f, 0.f, 0.f);
-        if (c < S) v[c] = ld_cluster4(mapa_shared(a, c));
+        if (c < S) v[c] = ld_cluster4(mapa_shared(own + at * 4, c));
       }
 #pragma unroll
       for (int c = 0; c < 8; ++c) w.x += v[c].x, w.y += v[c].y, w.z += v[c].z, w.w += v[c].w;
@@ -129,6 +125,7 @@ __device__ __forceinline__ void finish(const LinearParams& p, uint32_t own, int 
   const int end = min(quads, (rank + 1) * share);
   int e = rank * share + tid, tok = e / per, q = e - tok * per;
   const int step_tok = nthreads / per, step_q = nthreads - step_tok * per;
+#pragma unroll 2
   for (; e < end; e += nthreads, tok += step_tok, q += step_q) {
     if (q >= per) q -= per, ++tok;
     const int i = q * 4, n = n0 + i;

@@ -36,7 +36,7 @@ constexpr int kThreads = (kIssuer + kIssuers) * 32;
 constexpr int kRing = 13;                    // column tiles of an unpacking warp's ring
 constexpr int kStages = 4;                   // column tiles of codes in TMEM (64 columns each) and of token rows
 constexpr int kD = 4;                        // accumulators in TMEM, 64 columns each
-constexpr int kFar = 12;                     // column tiles of scales of a scaling warp's ring
+constexpr int kFar = 12;                     // column tiles of scales in shared memory
 constexpr int kLd = 128 + 4;                 // floats of one token's sums
 constexpr int kColsA = kD * 64;              // first TMEM column of the codes (all 512 are in use)
 
@@ -76,10 +76,10 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) & ~uintptr_t(1023));
   uint8_t* s_x = smem;                                        // [kStages][2][NP][128 bytes]
   uint8_t* s_ring = s_x + kStages * kXBytes;                  // [kUnpack][kRing][1024]
-  uint8_t* s_scales = s_ring + kUnpack * kRing * 1024;        // [kScale][kFar][2 row tiles][kGroups][32 bytes]
-  float* s_sums = reinterpret_cast<float*>(s_scales + kScale * kFar * kGroups * 64);  // [M][kLd]
+  uint8_t* s_scales = s_ring + kUnpack * kRing * 1024;        // [kFar][8 row tiles][kGroups][32 bytes]
+  float* s_sums = reinterpret_cast<float*>(s_scales + kFar * kGroups * 256);  // [M][kLd]
   // full: a column tile's codes are in TMEM and its token rows in shared memory; free: its products are done
-  __shared__ __align__(8) uint64_t full[kStages], free_[kStages], d_full[kD], d_empty[kD], drain[kIssuers];
+  __shared__ __align__(8) uint64_t full[kStages], free_[kStages], d_full[kD], d_empty[kD], s_full[kFar], drain[kIssuers];
   __shared__ uint32_t s_tmem;
   __shared__ int s_abort;
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
@@ -87,6 +87,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     s_abort = 0;
     for (int i = 0; i < kStages; ++i) mbar_init(full + i, kUnpack + 1), mbar_init(free_ + i, kByGroup ? kIssuers : 1);
     for (int i = 0; i < kD; ++i) mbar_init(d_full + i, 1), mbar_init(d_empty + i, kScale);
+    for (int i = 0; i < kFar; ++i) mbar_init(s_full + i, 32);
     for (int i = 0; i < kIssuers; ++i) mbar_init(drain + i, 1);
     fence_mbar_init();
     fence_async_smem();
@@ -175,40 +176,18 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     // ------------------------------------------------------------ scales and sums
     const int quad = warp & 3, row = quad * 32 + lane;
     const uint32_t from = tmem + ((uint32_t)(quad * 32) << 16);
-    // the scales of the warp's two row tiles: 64 bytes a group, 16 to a lane
-    constexpr int kBytes = kGroups * 64;
-    const uint32_t ring = smem_u32(s_scales) + (warp - kUnpack) * (kFar * kBytes);
-    int f_tile = tile0, f_i = 0, f_at = 0;
-    const uint8_t* sc = nullptr;
-    auto fetch = [&]() {
-      if (f_tile < p.tiles && n_kt > 0) {
-        if (f_i == 0)
-          sc = reinterpret_cast<const uint8_t*>(p.w.s) +
-               ((int64_t)row_tile(f_tile, 2 * quad + lane / (2 * kGroups) % 2) * p.w.groups + (int64_t)c0 * kGroups) * 32 +
-               lane % (2 * kGroups) * 16;
-        if (lane < 4 * kGroups) cp_async16(ring + f_at * kBytes + lane * 16, sc);
-        sc += kGroups * 32;
-        if (++f_i == n_kt) f_i = 0, f_tile += tile_step;
-      }
-      asm volatile("cp.async.commit_group;" ::: "memory");
-      if (++f_at == kFar) f_at = 0;
-    };
-    for (int i = 0; i < kFar - 1; ++i) fetch();
-    const uint32_t mine = ring + (lane >> 4) * (kGroups * 32) + (row & 7) * 4 + ((row >> 3) & 1) * 2;
-    int at = 0;
-    Pipe d;
+    const uint32_t mine = smem_u32(s_scales) + (row >> 4) * (kGroups * 32) + (row & 7) * 4 + ((row >> 3) & 1) * 2;
+    Pipe d, x;
     for (int tile = tile0; tile < p.tiles; tile += tile_step) {  // (all of them: the four warps meet at a barrier)
       float acc[NP];
 #pragma unroll
       for (int n = 0; n < NP; ++n) acc[n] = 0.f;
       for (int i = 0; i < n_kt; ++i) {
-        asm volatile("cp.async.wait_group %0;" ::"n"(kFar - 2) : "memory");
-        __syncwarp();
-        fetch();
+        wait(s_full + x.at, x.phase);
 #pragma unroll
         for (int g = 0; g < kGroups; ++g) {
           uint16_t h;
-          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(mine + at * kBytes + g * 32) : "memory");
+          asm volatile("ld.shared.u16 %0, [%1];" : "=h"(h) : "r"(mine + x.at * (kGroups * 256) + g * 32) : "memory");
           const float s = __half2float(__ushort_as_half(h));
           wait(d_full + d.at, d.phase);
           __syncwarp();
@@ -224,7 +203,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
           for (int n = 0; n < NP; ++n) acc[n] += s * __uint_as_float(v[n]);
           d.next<kD>();
         }
-        if (++at == kFar) at = 0;
+        x.next<kFar>();
       }
 #pragma unroll
       for (int n = 0; n < NP; ++n)
@@ -232,24 +211,44 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
       if (S == 1) {
         const int n0 = tile * p.outs;
         asm volatile("bar.sync 1, 128;" ::: "memory");
-        finish<1, kLd, 64>(p, smem_u32(s_sums), 1, 0, n0, p.swiglu ? (p.n_out + n0) & 15 : 0, tid - kUnpack * 32, kScale * 32);
+        finish<1, kLd, 64>(p, s_sums, 1, 0, n0, p.swiglu ? (p.n_out + n0) & 15 : 0, tid - kUnpack * 32, kScale * 32);
         asm volatile("bar.sync 1, 128;" ::: "memory");  // the sums are free again
       }
     }
-    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (warp == kLoader) {
-    // ------------------------------------------------------------ token rows
-    if (lane == 0) {
-      Pipe x;
-      for (int tile = tile0; tile < p.tiles && ok; tile += tile_step)
-        for (int i = 0; i < n_kt; ++i) {
-          if (!wait(free_ + x.at, x.phase ^ 1)) break;
+    // ------------------------------------------------------------ token rows and scales
+    // Scales go to a ring of their own, for a scaling warp may be kD groups behind the products, which may be kStages
+    // column tiles behind this warp: 16 bytes of a row tile's to a lane.
+    static_assert(kFar > kStages + kD, "a place is read before it is written again");
+    constexpr int kPieces = 16 * kGroups;  // of a column tile
+    Pipe x, s;
+    for (int tile = tile0; tile < p.tiles && ok; tile += tile_step) {
+      const uint8_t* sc[(kPieces + 31) / 32];
+#pragma unroll
+      for (int k = 0; k < (kPieces + 31) / 32; ++k) {
+        const int e = lane + 32 * k;
+        sc[k] = reinterpret_cast<const uint8_t*>(p.w.s) +
+                ((int64_t)row_tile(tile, min(e / (2 * kGroups), 7)) * p.w.groups + (int64_t)c0 * kGroups) * 32 + e % (2 * kGroups) * 16;
+      }
+      for (int i = 0; i < n_kt; ++i) {
+        if (!wait(free_ + x.at, x.phase ^ 1)) break;
+        __syncwarp();
+        if (lane == 0) {
           mbar_arrive_expect_tx(full + x.at, kXBytes);
           tma_load_2d(s_x + x.at * kXBytes, &xmap, full + x.at, (c0 + i) * 128, 0);
           tma_load_2d(s_x + x.at * kXBytes + kXBytes / 2, &xmap, full + x.at, (c0 + i) * 128 + 64, 0);
-          x.next<kStages>();
         }
+#pragma unroll
+        for (int k = 0; k < (kPieces + 31) / 32; ++k) {
+          if (lane + 32 * k < kPieces) cp_async16(smem_u32(s_scales) + s.at * (kGroups * 256) + (lane + 32 * k) * 16, sc[k]);
+          sc[k] += kGroups * 32;
+        }
+        asm volatile("cp.async.mbarrier.arrive.noinc.shared::cta.b64 [%0];" ::"r"(smem_u32(s_full + s.at)) : "memory");
+        x.next<kStages>();
+        s.next<kFar>();
+      }
     }
+    asm volatile("cp.async.wait_all;" ::: "memory");
   } else if (lane == 0) {
     // ------------------------------------------------------------ tensor cores
     constexpr uint32_t idesc = idesc_bf16_f32(128, NP, false, false);
@@ -294,7 +293,7 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   if (S > 1) {
     cluster_sync();
     const int n0 = tile0 * p.outs;
-    finish<1, kLd, 64>(p, smem_u32(s_sums), S, rank, n0, p.swiglu ? (p.n_out + n0) & 15 : 0, tid, kThreads);
+    finish<1, kLd, 64>(p, s_sums, S, rank, n0, p.swiglu ? (p.n_out + n0) & 15 : 0, tid, kThreads);
     cluster_sync();  // every CTA's sums are read before its shared memory goes
   }
   if (warp == kIssuer) {
@@ -309,7 +308,7 @@ static void launch(LinearParams& p, cudaStream_t st) {
   // SwiGLU: four gate tiles meet four up tiles, or three gate tiles four, where the up rows start inside a tile
   p.outs = !p.swiglu ? 128 : p.n_out % 16 == 0 ? 64 : 48;
   p.tiles = (p.n_out + p.outs - 1) / p.outs;
-  constexpr int kFixed = kStages * 2 * NP * 128 + kUnpack * kRing * 1024 + kScale * kFar * (8 / GS) * 64 + 1024;
+  constexpr int kFixed = kStages * 2 * NP * 128 + kUnpack * kRing * 1024 + kFar * (8 / GS) * 256 + 1024;
   cudaLaunchConfig_t cfg{};
   cfg.blockDim = dim3(kThreads);
   cfg.stream = st;
