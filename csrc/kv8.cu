@@ -440,8 +440,9 @@ __device__ __forceinline__ void blocks_of(const AttnParams& p, int b, int& len, 
 
 // s_pre[b]: steps (of kWarps blocks) before sequence b, for one KV head and group; returns their number. The host has
 // checked that all of them fit 30 bits.
-template <int kSides = 1>  // of kThreads threads
-__device__ __forceinline__ int prefix_steps(const AttnParams& p, int* s_pre, int* s_warp) {
+// kSides: of kThreads threads; each sequence's steps rounded up to a multiple of `unit`.
+template <int kSides = 1>
+__device__ __forceinline__ int prefix_steps(const AttnParams& p, int unit, int* s_pre, int* s_warp) {
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   int carry = 0;
   for (int b0 = 0; b0 < p.B; b0 += kThreads * kSides) {
@@ -450,6 +451,7 @@ __device__ __forceinline__ int prefix_steps(const AttnParams& p, int* s_pre, int
       int len, lo, first, count;
       blocks_of(p, b0 + tid, len, lo, first, count);
       n = (count + kWarps - 1) / kWarps;
+      if (unit > 1) n = (n + unit - 1) / unit * unit;
     }
     int x = n;
 #pragma unroll
@@ -471,7 +473,19 @@ __device__ __forceinline__ int prefix_steps(const AttnParams& p, int* s_pre, int
   }
   return carry;
 }
-__device__ __forceinline__ int steps_of_cta(int total, int ctas) { return max((total + ctas - 1) / ctas, kMinSteps); }
+// The ranges: `per` steps for each CTA; returns how many steps all segments take. Where segments are few beside the
+// CTAs, each starts a range of its own (its steps count as a multiple of `per`): a CTA that ends one segment and
+// begins another waits twice for page, scales and codes, 3 of 16 us for 16 x 2304.
+template <int kSides = 1>
+__device__ __forceinline__ int cut_ranges(const AttnParams& p, int V, int* s_pre, int* s_warp, int& per) {
+  int total = prefix_steps<kSides>(p, 1, s_pre, s_warp) * V;
+  const int segments = p.B * V;
+  const bool own = 3 * segments <= p.ctas;
+  const int ranges = own ? p.ctas - segments : p.ctas;
+  per = max((total + ranges - 1) / ranges, kMinSteps);
+  if (own) total = prefix_steps<kSides>(p, per, s_pre, s_warp) * V;
+  return total;
+}
 // The last sequence that starts at or before step `at` of all.
 __device__ __forceinline__ int sequence_at(const int* s_pre, int B, int V, int at) {
   int b = 0, hi = B;
@@ -512,8 +526,7 @@ __global__ void __launch_bounds__(kThreads, 2) attn_kernel(AttnParams p) {
 
   int at = 0, end = 1, per = 1, b = blockIdx.x / V;
   if (p.ctas > 0) {
-    const int total = prefix_steps(p, s_pre, s_warp) * V;
-    per = steps_of_cta(total, p.ctas);
+    const int total = cut_ranges(p, V, s_pre, s_warp, per);
     at = blockIdx.x * per;
     end = min(total, at + per);
     if (at < end) b = sequence_at(s_pre, p.B, V, at);
@@ -808,8 +821,8 @@ __global__ void __launch_bounds__(kThreads * kSides) join_kernel(AttnParams p) {
   __shared__ float4 s_acc[kSides == 2 ? kThreads : 1], s_ml[kSides == 2 ? kThreads : 1];
   const int tid = threadIdx.x, side = tid / kThreads, warp = tid / 32 % kWarps, lane = tid & 31, r = lane >> 2, t = lane & 3;
   const int V = p.m.Hkv * p.hg;
-  const int total = prefix_steps<kSides>(p, s_pre, s_warp) * V;
-  const int per = steps_of_cta(total, p.ctas);
+  int per;
+  const int total = cut_ranges<kSides>(p, V, s_pre, s_warp, per);
   const int cut = ((int)blockIdx.x + 1) * per;
   bool mine = cut < total;
   int b = 0, v = 0, np = 0;
