@@ -100,7 +100,6 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
     return min(p.swiglu && rt >= 4 ? ((p.n_out + n0) >> 4) + rt - 4 : (n0 >> 4) + rt, (p.w.N + 15) / 16 - 1);
   };
   asm volatile("griddepcontrol.wait;" ::: "memory");
-  asm volatile("griddepcontrol.launch_dependents;");
   if (warp == kIssuer) {
     tmem_alloc(&s_tmem, 512);
     tmem_relinquish();
@@ -108,6 +107,8 @@ __global__ void __launch_bounds__(kThreads, 1) linear_kernel(const __grid_consta
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
+  // Not before TMEM is held: a kernel that begins now may take TMEM and then wait for this one to end.
+  asm volatile("griddepcontrol.launch_dependents;");
   const uint32_t tmem = s_tmem;
   bool ok = true;
   auto wait = [&](uint64_t* bar, uint32_t phase) {
