@@ -93,7 +93,8 @@ struct AppendParams {
 // q heads need no block: a warp turns kTok tokens of one head after another and
 // keeps the tokens' angles in registers. Bound by the bytes of qkv and out while
 // blocks are many; a few tokens are spread over more CTAs (latency is all there
-// is).
+// is). Measured, 28 + 2 * 4 heads of D 128: 8 x 2048 tokens in 54.5 us (285 MB at
+// 5.2 TB/s, 0.80 of a copy's rate; 64 x 4096: 6.1 TB/s), 64 single tokens in 5.6.
 constexpr int kAppendWarps = 8;
 
 template <int D>
@@ -277,7 +278,8 @@ struct GatherParams {
 // out = code * scale, rounded once: a thread keeps its head and its 16 dims and
 // turns kGatherRows positions, all loaded before the first is stored. Bound by
 // the bytes moved; a position's heads are one run of the output, and 128 bytes
-// of a head's row one line of the pool.
+// of a head's row one line of the pool. Measured, 4 heads of D 128: 64 x 4096
+// positions in 75 us (403 MB at 5.4 TB/s, 0.82 of a copy's rate).
 constexpr int kGatherThreads = 256;
 constexpr int kGatherRows = 2;
 
@@ -349,6 +351,15 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(GatherParams p) 
 // through the workspace to a second kernel, which joins them in order; it has its
 // prefix sums ready when the first one ends (joined by the last CTA to arrive,
 // 37 parts took 8 us of fences, waits and loads).
+//
+// Measured, 28 query heads of 4 KV heads, D 128, pages of 64: 64 x 4096 keys in
+// 50.5 us (5.34 TB/s, 0.81 of a copy's rate: 16 warps a SM with a step of K and V
+// each in registers keep 64 KB in flight, and the tensor pipe is busy for a sixth
+// of the time); 1 x 100001 keys, 8 KV heads, in 45 us (0.69: a range more or less
+// of 128 keys is 4 % of a CTA's work, and the join adds 3 us); 16 ragged sequences
+// of up to 2304 keys in 14.5 us and 1 x 97 keys in 4.5 us, the chain page -> codes
+// -> products -> sums of eight warps. A ring of asynchronous copies in shared
+// memory adds instructions and was slower (63 us for 64 x 4096, this form then 55).
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWarps = 8;
 constexpr int kThreads = kWarps * 32;
