@@ -368,9 +368,9 @@ at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_
   p.swiglu = swiglu;
   p.status = device_status_word();
   auto st = at::cuda::getCurrentCUDAStream();
-  // Here every group of eight rows costs its products and sums again; on tcgen05 32 rows cost what one does. Both at
-  // 16 and at 24 rows: 3584 -> 3584 7.6 us here, 8.7 there and 13.5, 8.8; 18944 -> 3584 (groups of 64) 18.0, 25.7 and
-  // 41.1, 25.9; 3584 -> 37888 SwiGLU 24.7, 31.4 and 36.2, 32.4 (groups of 32: 26.2, 51.2 and 39.4, 52.2).
+  // Here every group of eight rows costs its products and sums again; on tcgen05 32 rows cost what one does (17 or 24
+  // rows there; 16 and 24 here): 3584 -> 3584 8.3 us; 7.5 and 13.5; 18944 -> 3584, groups of 64, 28; 18 and 41;
+  // 3584 -> 37888 SwiGLU 30.5; 24.9 and 36 (groups of 32, the one that would gain from a later change: 52; 26 and 39).
   if (M <= 8)
     launch_group<1>(p, st);
   else if (M <= 16)
