@@ -83,6 +83,15 @@ def test_gpu_linear_more_row_tiles_than_sms(group):
     check("cuda", 20, 128 * 330 + 7, 384, group, bias=True)
 
 
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,group", [(96, 32), (128, 128), (640, 64), (1152, 128)])
+def test_gpu_linear_rings_across_row_tiles(K, group):
+    """Columns that a warp's turns, the scales' stages and a row tile's end cut
+    in other places for each row tile."""
+    check("cuda", 50, 128 * 200 + 9, K, group)
+    check("cuda", 18, 2 * (64 * 170 + 8), K, group, swiglu=True)
+
+
 @pytest.mark.parametrize("dev", CPU_GPU)
 @pytest.mark.parametrize("M,N,K,bias,residual,swiglu", [(1, 200, 256, True, True, False), (4, 2 * 133, 512, False, False, True),
                                                         (16, 2 * 64, 384, True, False, True), (33, 130, 640, True, True, False),
