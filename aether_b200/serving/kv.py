@@ -98,6 +98,7 @@ class PagedKVCache:
         self.alloc = PageAllocator(num_pages, page_size, reserved=1)
         self.table = torch.zeros(rows, self.max_pages, dtype=torch.int32, device=device)
         self.pages: list = [[] for _ in range(rows)]
+        self._changed: set = set()  # rows whose pages have changed since take_changes()
         self.device = torch.device(device)
 
     def _make_pools(self, n_layers: int, num_pages: int, n_kv_heads: int, head_dim: int, device) -> None:
@@ -114,6 +115,7 @@ class PagedKVCache:
     def _write_row(self, row: int, start: int) -> None:
         new = self.pages[row][start:]
         if new:
+            self._changed.add(row)
             self.table[row, start : start + len(new)].copy_(torch.tensor(new, dtype=torch.int32), non_blocking=False)
 
     def match_prefix(self, row: int, tokens: list) -> int:
@@ -150,7 +152,25 @@ class PagedKVCache:
         for p in self.pages[row]:
             self.alloc.release(p)
         self.pages[row] = []
+        self._changed.add(row)
         self.table[row].zero_()
+
+    # ---- one cache's bookkeeping followed by its copies (tensor-parallel ranks hold the same pages of other heads)
+    def take_changes(self) -> list:
+        """[(row, pages)] of the rows changed since the last call."""
+        rows, self._changed = sorted(self._changed), set()
+        return [(r, list(self.pages[r])) for r in rows]
+
+    def apply_changes(self, changes) -> None:
+        """Sets the table rows that another cache's ``take_changes`` names; this
+        cache's own allocator is not asked and must not be used beside it."""
+        for row, pages in changes:
+            if not 0 <= row < self.rows or len(pages) > self.max_pages or not all(0 < p < self.alloc.num_pages for p in pages):
+                raise ValueError(f"page table row {row}: not one of this cache's rows and pages")
+            host = torch.zeros(self.max_pages, dtype=torch.int32)
+            host[: len(pages)] = torch.tensor(pages, dtype=torch.int32)
+            self.pages[row] = list(pages)
+            self.table[row].copy_(host)
 
 
 class Paged8KVCache(PagedKVCache):
