@@ -693,13 +693,16 @@ void gemm_bf16(at::Tensor a, at::Tensor b, at::Tensor out, bool a_mn, bool b_mn,
     p.alpha_ptr = alpha_t->data_ptr<float>();
   }
   if (bias && bias->defined()) {
-    TORCH_CHECK(bias->scalar_type() == at::kBFloat16 && bias->numel() == N && bias->is_contiguous(), "gemm_bf16: bias must be bf16 [N]");
+    TORCH_CHECK(bias->device() == a.device() && bias->scalar_type() == at::kBFloat16 && bias->numel() == N &&
+                    bias->is_contiguous() && reinterpret_cast<uintptr_t>(bias->data_ptr()) % 16 == 0,
+                "gemm_bf16: bias must be bf16 [N] beside the operands, on a 16-byte boundary");
     p.bias = reinterpret_cast<const __nv_bfloat16*>(bias->data_ptr());
   }
   if (residual && residual->defined()) {
-    TORCH_CHECK(residual->scalar_type() == at::kBFloat16 && residual->size(0) == M && residual->size(1) == N &&
-                    residual->stride(1) == 1 && residual->stride(0) % 8 == 0,
-                "gemm_bf16: residual must be bf16 [M, N]");
+    TORCH_CHECK(residual->device() == a.device() && residual->scalar_type() == at::kBFloat16 && residual->dim() == 2 &&
+                    residual->size(0) == M && residual->size(1) == N && residual->stride(1) == 1 &&
+                    residual->stride(0) % 8 == 0 && reinterpret_cast<uintptr_t>(residual->data_ptr()) % 16 == 0,
+                "gemm_bf16: residual must be bf16 [M, N] beside the operands, rows on 16-byte boundaries");
     p.residual = reinterpret_cast<const __nv_bfloat16*>(residual->data_ptr());
     p.ldr = residual->stride(0);
   }
