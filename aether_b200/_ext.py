@@ -24,6 +24,7 @@ _KERNELS_PER_CALL = {
     "layernorm_bwd": 3,
     "attention_bwd": 3,
     "grad_norm": 2,
+    "linear_w4_output": 0,
     "read_and_clear_status": 0,
 }
 

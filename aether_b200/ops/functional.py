@@ -943,31 +943,56 @@ def dequant_w4(w, out=None):
     return out
 
 
+def _on_16_bytes(t):
+    """Whether bf16 rows start on 16-byte boundaries and do not overlap (as tensor maps want them)."""
+    return t.data_ptr() % 16 == 0 and (t.dim() == 1 or (t.stride(0) % 8 == 0 and t.stride(0) >= t.shape[1]))
+
+
+def _to_16_bytes(t):
+    return t if t is None or _on_16_bytes(t) else t.clone(memory_format=torch.contiguous_format)
+
+
 def linear_w4(x, w, bias=None, residual=None, swiglu=False, out=None):
     """y = x @ w^T (+ bias) (+ residual) for x bf16 [M, K] and a W4Weight [N, K];
     swiglu: w = [gate; up] and y = silu(gate) * up, [M, N / 2]. Up to W4_ROWS
     rows the 4-bit weights are multiplied as they are (exact codes, fp32 sums and
-    scales); more rows expand them to bf16 for the tensor-core GEMM."""
+    scales, one rounding of y). More rows expand them for the tensor-core GEMM,
+    which takes bf16: each weight is rounded once, and SwiGLU, a kernel of its
+    own, rounds gate, up, their product and the sum with the residual (the steps
+    of the framework's bf16 FFN). Where N or y's width is no multiple of 8 that
+    GEMM cannot write y, and W4_ROWS rows at a time are taken as they are."""
     M = x.shape[0]
     if M <= W4_ROWS and _cuda(x):
         return C().linear_w4(x, w.q, w.s, w.N, w.K, w.group, bias, residual, swiglu, out)
-    if out is None:
-        out = torch.empty(M, w.N // 2 if swiglu else w.N, dtype=BF16, device=x.device)
     if _cuda(x):
+        out = C().linear_w4_output(x, w.q, w.s, w.N, w.K, w.group, bias, residual, swiglu, out)
         if w.N % 8 == 0 and out.shape[1] % 8 == 0:
-            wb = dequant_w4(w)
+            wb, x, bias = dequant_w4(w), _to_16_bytes(x), _to_16_bytes(bias)
             if swiglu:
-                out.copy_(swiglu_residual(gemm(x, wb, bias=bias), residual))
+                a = swiglu_residual(gemm(x, wb, bias=bias), residual)
             else:
-                gemm(x, wb, bias=bias, residual=residual, out=out)
+                a = out if _on_16_bytes(out) else torch.empty(M, w.N, dtype=BF16, device=x.device)
+                gemm(x, wb, bias=bias, residual=_to_16_bytes(residual), out=a)
+            if a is not out:
+                out.copy_(a)
         else:
             for i in range(0, M, W4_ROWS):
                 r = slice(i, min(M, i + W4_ROWS))
                 C().linear_w4(x[r], w.q, w.s, w.N, w.K, w.group, bias, None if residual is None else residual[r],
                               swiglu, out[r])
         return out
+    n_out = w.N // 2 if swiglu else w.N
     if x.dim() != 2 or x.shape[1] != w.K:
         raise ValueError("linear_w4: x is [M, K]")
+    if swiglu and w.N % 2:
+        raise ValueError("linear_w4: SwiGLU takes an even number of rows (gate, then up)")
+    if bias is not None and bias.shape != (w.N,):
+        raise ValueError("linear_w4: bias is [N]")
+    for t, name in ((residual, "residual"), (out, "out")):
+        if t is not None and t.shape != (M, n_out):
+            raise ValueError(f"linear_w4: {name} is [M, N] (SwiGLU: [M, N / 2])")
+    if out is None:
+        out = torch.empty(M, n_out, dtype=BF16)
     y = x.float() @ ref.w4_values(w.q, w.s, w.N, w.K, w.group).t()
     if bias is not None:
         y = y + bias.float()

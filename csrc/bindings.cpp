@@ -77,6 +77,9 @@ at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::
 at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group,
                      std::optional<at::Tensor> bias, std::optional<at::Tensor> residual, bool swiglu,
                      std::optional<at::Tensor> out);
+at::Tensor linear_w4_output(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group,
+                            std::optional<at::Tensor> bias, std::optional<at::Tensor> residual, bool swiglu,
+                            std::optional<at::Tensor> out);
 void dequant_w4(at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group, at::Tensor out);
 // gemm_skinny.cu
 void skinny_gemm(at::Tensor x, at::Tensor w, at::Tensor acc, int64_t splits, int64_t acc_mc,
@@ -246,6 +249,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("gather_kv8", &aether::gather_kv8, "8-bit paged cache rows -> bf16");
   m.def("kv8_decode_attention", &aether::kv8_decode_attention, "single-token attention over an 8-bit paged cache");
   m.def("linear_w4", &aether::linear_w4, "a few rows times 4-bit weights with group scales");
+  m.def("linear_w4_output", &aether::linear_w4_output, "checks linear_w4's arguments for any number of rows; its output");
   m.def("dequant_w4", &aether::dequant_w4, "4-bit weights with group scales -> bf16");
   m.def("read_and_clear_status", &aether::read_and_clear_status,
         "Returns (and clears) the device status word set by kernels whose bounded waits expired");

@@ -325,23 +325,23 @@ static Weight make_weight(const at::Tensor& q, const at::Tensor& s, int64_t N, i
 
 }  // namespace w4
 
-at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group,
-                     std::optional<at::Tensor> bias, std::optional<at::Tensor> residual, bool swiglu,
-                     std::optional<at::Tensor> out) {
-  using namespace w4;
-  LinearParams p{};
+namespace w4 {
+// Checks the arguments of a product of any number of rows and fills p with them; returns the output, made where none is
+// given.
+static at::Tensor arguments(LinearParams& p, const at::Tensor& x, const at::Tensor& q, const at::Tensor& s, int64_t N,
+                            int64_t K, int64_t group, const std::optional<at::Tensor>& bias,
+                            const std::optional<at::Tensor>& residual, bool swiglu, const std::optional<at::Tensor>& out) {
   p.w = make_weight(q, s, N, K, group, "linear_w4");
   TORCH_CHECK(x.dim() == 2, "linear_w4: x is [M, K]");
   const int64_t M = x.size(0), n_out = swiglu ? N / 2 : N;
   TORCH_CHECK(!swiglu || N % 2 == 0, "linear_w4: SwiGLU takes an even number of rows (gate, then up)");
-  TORCH_CHECK(x.device() == q.device() && x.scalar_type() == at::kBFloat16 && x.dim() == 2 && x.size(1) == K &&
-                  x.stride(1) == 1,
+  TORCH_CHECK(x.device() == q.device() && x.scalar_type() == at::kBFloat16 && x.size(1) == K && x.stride(1) == 1,
               "linear_w4: x is bf16 [M, K] with unit inner stride, beside the weights");
+  TORCH_CHECK(M < (int64_t(1) << 31), "linear_w4: fewer than 2^31 rows");
   const at::Tensor y = out && out->defined() ? *out : at::empty({M, n_out}, x.options());
   TORCH_CHECK(y.device() == q.device() && y.scalar_type() == at::kBFloat16 && y.dim() == 2 && y.size(0) == M &&
                   y.size(1) == n_out && (n_out == 1 || y.stride(1) == 1),
               "linear_w4: out is bf16 [M, N] (SwiGLU: [M, N / 2]) with unit inner stride, beside the weights");
-  TORCH_CHECK(M <= 64, "linear_w4: at most 64 rows");
   if (bias && bias->defined()) {
     TORCH_CHECK(bias->device() == q.device() && bias->scalar_type() == at::kBFloat16 && bias->is_contiguous() &&
                     bias->numel() == N,
@@ -355,17 +355,36 @@ at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_
     p.res = reinterpret_cast<const __nv_bfloat16*>(residual->data_ptr());
     p.rs = residual->stride(0);
   }
+  p.y = reinterpret_cast<__nv_bfloat16*>(y.data_ptr());
+  p.ys = y.stride(0);
+  p.M = (int)M;
+  p.n_out = (int)n_out;
+  p.swiglu = swiglu;
+  return y;
+}
+}  // namespace w4
+
+at::Tensor linear_w4_output(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group,
+                            std::optional<at::Tensor> bias, std::optional<at::Tensor> residual, bool swiglu,
+                            std::optional<at::Tensor> out) {
+  w4::LinearParams p{};
+  return w4::arguments(p, x, q, s, N, K, group, bias, residual, swiglu, out);
+}
+
+at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group,
+                     std::optional<at::Tensor> bias, std::optional<at::Tensor> residual, bool swiglu,
+                     std::optional<at::Tensor> out) {
+  using namespace w4;
+  LinearParams p{};
+  const at::Tensor y = arguments(p, x, q, s, N, K, group, bias, residual, swiglu, out);
+  const int64_t M = x.size(0);
+  TORCH_CHECK(M <= 64, "linear_w4: at most 64 rows");
   if (M == 0) return y;
   c10::cuda::CUDAGuard g(q.device());
   // 16-byte copies: rows on 16-byte boundaries
   if (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0 || (M > 1 && x.stride(0) % 8 != 0)) x = x.clone(at::MemoryFormat::Contiguous);
   p.x = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr());
   p.xs = x.stride(0);
-  p.y = reinterpret_cast<__nv_bfloat16*>(y.data_ptr());
-  p.ys = y.stride(0);
-  p.M = (int)M;
-  p.n_out = (int)n_out;
-  p.swiglu = swiglu;
   p.status = device_status_word();
   auto st = at::cuda::getCurrentCUDAStream();
   // Here every group of eight rows costs its products and sums again; on tcgen05 32 rows cost what one does (17 or 24
