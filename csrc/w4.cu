@@ -381,8 +381,9 @@ at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_
   TORCH_CHECK(M <= 64, "linear_w4: at most 64 rows");
   if (M == 0) return y;
   c10::cuda::CUDAGuard g(q.device());
-  // 16-byte copies: rows on 16-byte boundaries
-  if (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0 || (M > 1 && x.stride(0) % 8 != 0)) x = x.clone(at::MemoryFormat::Contiguous);
+  // 16-byte copies: rows on 16-byte boundaries; a tensor map (more than 16 rows) wants rows that do not overlap
+  if (reinterpret_cast<uintptr_t>(x.data_ptr()) % 16 != 0 || (M > 1 && x.stride(0) % 8 != 0) || (M > 16 && x.stride(0) < K))
+    x = x.clone(at::MemoryFormat::Contiguous);
   p.x = reinterpret_cast<const __nv_bfloat16*>(x.data_ptr());
   p.xs = x.stride(0);
   p.status = device_status_word();
