@@ -163,6 +163,8 @@ def main():
                     help="4-bit projections with a scale for each GROUP columns (32, 64 or 128; one GPU)")
     ap.add_argument("--kv-bits", type=int, default=16, choices=[8, 16], help="8: paged KV cache in 8 bits")
     args = ap.parse_args()
+    if args.w4 and (args.tp > 1 or args.emulate_tp > 1 or int(os.environ.get("WORLD_SIZE", "1")) > 1):
+        ap.error("--w4 measures one GPU (the TP shards are bf16)")
     _ext.C()
     batches = [int(b) for b in (args.batches or ("1,8,32" if args.model == "1.5b" else "1,16,64")).split(",")]
     prompt = args.prompt or (512 if args.model == "1.5b" else 2048)

@@ -226,7 +226,8 @@ class QwenWeights:
         """Replaces the four projections of every layer by 4-bit codes with a
         scale for each ``group`` columns (``ops.functional.W4Weight``); decode
         multiplies them as they are, prefill expands them before each GEMM.
-        Embeddings, LM head, norms and biases stay bf16."""
+        Embeddings, LM head, norms and biases stay bf16. Before a model is built
+        on the weights: its captured graphs keep the tensors that they replace."""
         if self.tp_size > 1:
             raise ValueError("4-bit projections serve one GPU (the TP shards are bf16)")
         for ws in (self.wqkv, self.wo, self.wgu, self.wd):
@@ -302,6 +303,9 @@ class QwenModel:
         tp_rank = tp.rank if tp is not None else 0
         tp_size = tp.world if tp is not None else 1
         self.w = weights or QwenWeights(cfg, device, seed, tp_rank, tp_size)
+        if tp is not None and (self.w.tp_rank, self.w.tp_size) != (tp_rank, tp_size):
+            raise ValueError(f"weights of rank {self.w.tp_rank} of {self.w.tp_size} for rank {tp_rank} of {tp_size}: the ranks' "
+                             "products are summed, so each needs its own shard (QwenWeights.shard)")
         self.hq, self.hkv, self.f = self.w.hq, self.w.hkv, self.w.f
         # vocabulary-parallel head: needs the TP object's merge / gather and a sharded head
         self.vp = (tp is not None and hasattr(tp, "vocab_argmax")
