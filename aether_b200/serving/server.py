@@ -305,6 +305,10 @@ def main():
         if not args.tokenizer and os.path.exists(os.path.join(args.hf, "tokenizer.json")):
             tok = BPETokenizer.from_file(os.path.join(args.hf, "tokenizer.json"))
         template = JinjaChatTemplate.from_hf_dir(args.hf) or template
+    if (args.w4 or args.kv_bits == 8) and isinstance(cfg, (DeepSeekConfig, MoEConfig)):
+        raise SystemExit("--w4 and --kv-bits 8 serve the dense models")
+    if args.w4 and args.tp > 1:
+        raise SystemExit("--w4 serves one GPU (the TP shards are bf16)")
     tp = None
     if args.tp > 1:  # one process per GPU; every rank builds its shard, rank 0 serves
         import torch.distributed as dist
@@ -328,8 +332,6 @@ def main():
         model = MoEQwenModel(cfg, device=args.device, max_batch=args.max_concurrent, max_seq=args.max_seq, tp=tp)
     else:
         if args.w4:
-            if args.tp > 1:
-                raise SystemExit("--w4 serves one GPU (the TP shards are bf16)")
             weights = (weights or QwenWeights(cfg, args.device)).quantize_w4(args.w4)
         pages = args.max_concurrent * -(-args.max_seq // 64) + 1 if args.kv_bits == 8 else 0
         model = QwenModel(cfg, device=args.device, max_batch=args.max_concurrent, max_seq=args.max_seq,
