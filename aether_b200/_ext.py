@@ -18,12 +18,16 @@ except Exception as e:  # noqa: BLE001
 
 
 # Kernel launches issued per extension call (for the launch count a benchmark
-# reports over its timed region).
+# reports over its timed region): a number, or a function of the module and the
+# call's arguments.
 _KERNELS_PER_CALL = {
     "rmsnorm_bwd": 2,
     "layernorm_bwd": 3,
     "attention_bwd": 3,
     "grad_norm": 2,
+    "kv8_decode_attention": lambda mod, q, kc, ks, vc, vs, table, slot, seqlen, out, Hq, scale, ws, window, cap:
+        mod.kv8_decode_kernels(q, kc, table, window),
+    "kv8_decode_kernels": 0,
     "linear_w4_output": 0,
     "read_and_clear_status": 0,
 }
@@ -31,8 +35,8 @@ _KERNELS_PER_CALL = {
 
 class _CountingModule:
     """Proxy over ``_C`` that counts kernel launches while counting is on.
-    Functions are kept as attributes once looked up: bare while counting is
-    off, wrapped while it is on."""
+    A function is wrapped when it is first looked up and kept as an attribute,
+    so later calls do not come through ``__getattr__``."""
 
     def __init__(self, mod):
         self._mod = mod
@@ -43,19 +47,15 @@ class _CountingModule:
         fn = getattr(self._mod, name)
         if not callable(fn):
             return fn
-        if self.enabled:
-            bare, k = fn, _KERNELS_PER_CALL.get(name, 1)
+        k = _KERNELS_PER_CALL.get(name, 1)
 
-            def fn(*a, **kw):
-                self.launches += k
-                return bare(*a, **kw)
+        def call(*a, **kw):
+            if self.enabled:
+                self.launches += k(self._mod, *a, **kw) if callable(k) else k
+            return fn(*a, **kw)
 
-        setattr(self, name, fn)  # found without this method from now on
-        return fn
-
-    def count(self, enable: bool) -> None:
-        if enable != self.enabled:
-            self.__dict__ = {"_mod": self._mod, "enabled": enable, "launches": self.launches}
+        setattr(self, name, call)
+        return call
 
 
 _PROXY = _CountingModule(_C) if _C is not None else None
@@ -68,7 +68,7 @@ def count_launches(enable: bool) -> int:
     n = _PROXY.launches
     if enable:
         _PROXY.launches = 0
-    _PROXY.count(enable)
+    _PROXY.enabled = enable
     return n
 
 

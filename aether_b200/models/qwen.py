@@ -723,7 +723,8 @@ class QwenModel:
 
     def _decode_body_unfused(self, B: int) -> None:
         """Decode step with separate norm / RoPE / combine kernels (13 per layer;
-        8 with 4-bit projections and an 8-bit cache)."""
+        with 4-bit projections and an 8-bit cache 9, or 8 where the page table
+        or the window spans at most 1024 keys)."""
         cfg, w, b = self.cfg, self.w, self.buf
         D = cfg.head_dim
         x, x2, h = b["x"][:B], b["x2"][:B], b["h"][:B]

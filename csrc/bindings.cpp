@@ -73,6 +73,7 @@ at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::
                                 at::Tensor page_table, at::Tensor slot, at::Tensor seqlen,
                                 std::optional<at::Tensor> into, int64_t Hq, double scale, at::Tensor workspace,
                                 int64_t window, double softcap);
+int64_t kv8_decode_kernels(at::Tensor q, at::Tensor kc, at::Tensor page_table, int64_t window);
 // w4.cu
 at::Tensor linear_w4(at::Tensor x, at::Tensor q, at::Tensor s, int64_t N, int64_t K, int64_t group,
                      std::optional<at::Tensor> bias, std::optional<at::Tensor> residual, bool swiglu,
@@ -248,6 +249,7 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("rope_kv8_append", &aether::rope_kv8_append, "RoPE, 8-bit quantisation and append to a paged cache");
   m.def("gather_kv8", &aether::gather_kv8, "8-bit paged cache rows -> bf16");
   m.def("kv8_decode_attention", &aether::kv8_decode_attention, "single-token attention over an 8-bit paged cache");
+  m.def("kv8_decode_kernels", &aether::kv8_decode_kernels, "kernels that kv8_decode_attention launches for these shapes");
   m.def("linear_w4", &aether::linear_w4, "a few rows times 4-bit weights with group scales");
   m.def("linear_w4_output", &aether::linear_w4_output, "checks linear_w4's arguments for any number of rows; its output");
   m.def("dequant_w4", &aether::dequant_w4, "4-bit weights with group scales -> bf16");

@@ -1070,6 +1070,19 @@ at::Tensor gather_kv8(at::Tensor codes, at::Tensor scale, at::Tensor page_table,
   return out;
 }
 
+namespace kv8 {
+// The most keys that a call can see of one sequence (with a window: that and the rest of its first block).
+static int64_t most_keys(const at::Tensor& kc, const at::Tensor& page_table, int64_t window) {
+  const int64_t keys = page_table.size(1) * kc.size(2);
+  return window > 0 ? std::min<int64_t>(keys, window + kBlock) : keys;
+}
+}  // namespace kv8
+
+// Kernels that kv8_decode_attention launches for these shapes.
+int64_t kv8_decode_kernels(at::Tensor q, at::Tensor kc, at::Tensor page_table, int64_t window) {
+  return q.size(0) == 0 ? 0 : kv8::most_keys(kc, page_table, window) <= kv8::kWholeKeys ? 1 : 2;
+}
+
 at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::Tensor vc, at::Tensor vs,
                                 at::Tensor page_table, at::Tensor slot, at::Tensor seqlen,
                                 std::optional<at::Tensor> into, int64_t Hq, double scale, at::Tensor workspace,
@@ -1119,8 +1132,7 @@ at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::
     p.cap_out = (float)softcap * kLog2e;
   }
   p.status = device_status_word();
-  int64_t keys = (int64_t)p.m.cols << p.m.shift;
-  if (window > 0) keys = std::min<int64_t>(keys, window + kBlock);
+  const int64_t keys = most_keys(kc, page_table, window);
   const int64_t most = B * Hkv * hg * std::max<int64_t>(1, (keys + kWarps * kBlock - 1) / (kWarps * kBlock));
   TORCH_CHECK(most < (int64_t(1) << 30), "kv8_decode_attention: the page table's positions times sequences and heads");
   // short tables: a CTA for each segment; else equal ranges for two CTAs an SM
