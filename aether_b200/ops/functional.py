@@ -798,6 +798,18 @@ def _kv8_rows(x, name):
     return x
 
 
+def _kv8_pages(codes, page_table, slot, n, name):
+    """CPU: the physical pages of positions 0 .. n of a table row, as far as the
+    row goes. Whatever is out of range raises here; the kernels report it in the
+    device status word."""
+    if not 0 <= slot < page_table.shape[0]:
+        raise IndexError(f"{name}: page-table row {slot} of {page_table.shape[0]}")
+    pages = page_table[slot, : -(-n // codes.shape[2])].long()
+    if pages.numel() and not 0 <= int(pages.min()) <= int(pages.max()) < codes.shape[0]:
+        raise IndexError(f"{name}: page-table row {slot} names a page outside the pool's {codes.shape[0]}")
+    return pages
+
+
 def rope_kv8_append(qkv, pos, slot, cos_t, sin_t, kc, ks, vc, vs, page_table, Hq, row_start=None, out=None):
     """Rotates the q and k heads of qkv [T, >= (Hq + 2 Hkv) D] and appends k and v
     to an 8-bit paged cache: codes uint8 [pages, Hkv, page, D] (code + 128) and
@@ -823,11 +835,13 @@ def rope_kv8_append(qkv, pos, slot, cos_t, sin_t, kc, ks, vc, vs, page_table, Hq
         r0, r1 = (b, b + 1) if row_start is None else (int(row_start[b]), int(row_start[b + 1]))
         if int(slot[b]) < 0 or r1 <= r0:
             continue
-        p0 = int(pos[b])
+        p0, p1 = int(pos[b]), int(pos[b]) + r1 - r0
+        pages = _kv8_pages(kc, page_table, int(slot[b]), p1, "rope_kv8_append")
+        if r0 < 0 or r1 > qkv.shape[0] or p0 < 0 or p1 > min(cos_t.shape[0], page_table.shape[1] * kc.shape[2]):
+            raise IndexError("rope_kv8_append: rows outside qkv, or positions outside the tables")
         x = qkv[r0:r1].float()
-        y = ref.rope(x, torch.arange(p0, p0 + r1 - r0), cos_t, sin_t, Hq + Hkv, D)
+        y = ref.rope(x, torch.arange(p0, p1), cos_t, sin_t, Hq + Hkv, D)
         heads = y[:, : (Hq + 2 * Hkv) * D].view(r1 - r0, Hq + 2 * Hkv, D)
-        pages = page_table[int(slot[b])]
         ref.kv8_store(heads[:, Hq : Hq + Hkv], p0, kc, ks, pages)
         ref.kv8_store(heads[:, Hq + Hkv :], p0, vc, vs, pages)
         out[r0:r1, : (Hq + Hkv) * D] = y[:, : (Hq + Hkv) * D].to(out.dtype)
@@ -846,7 +860,9 @@ def gather_kv8(codes, scale, page_table, slot, first, n, out=None):
         out = torch.empty(slot.shape[0], n, codes.shape[1], codes.shape[3], dtype=BF16)
     for b in range(slot.shape[0]):
         f = int(first[b]) if isinstance(first, torch.Tensor) else int(first)
-        v = ref.kv8_values(codes, scale, page_table[int(slot[b])], f + n)[f:]
+        if f < 0:
+            raise ValueError("gather_kv8: positions")
+        v = ref.kv8_values(codes, scale, _kv8_pages(codes, page_table, int(slot[b]), f + n, "gather_kv8"), f + n)[f:]
         out[b].zero_()
         out[b, : v.shape[0]] = v.to(BF16)
     return out
@@ -866,6 +882,8 @@ def kv8_decode_attention(q, kc, ks, vc, vs, page_table, slot, seqlen, Hq, scale,
         return C().kv8_decode_attention(q, kc, ks, vc, vs, page_table, slot, seqlen, out, Hq, scale, workspace, window,
                                         softcap)
     _kv8_rows(q, "kv8_decode_attention: q")
+    if window < 0 or not 0.0 <= softcap < float("inf"):
+        raise ValueError("kv8_decode_attention: window and softcap")
     D = kc.shape[3]
     if out is None:
         out = torch.empty(q.shape[0], Hq * D, dtype=BF16)
@@ -874,7 +892,10 @@ def kv8_decode_attention(q, kc, ks, vc, vs, page_table, slot, seqlen, Hq, scale,
         if L <= 0 or s < 0:
             out[b, : Hq * D] = 0
             continue
-        k, v = (ref.kv8_values(c, z, page_table[s], L)[None] for c, z in ((kc, ks), (vc, vs)))
+        pages = _kv8_pages(kc, page_table, s, L, "kv8_decode_attention")
+        if L > page_table.shape[1] * kc.shape[2]:
+            raise IndexError("kv8_decode_attention: more keys than the page table holds")
+        k, v = (ref.kv8_values(c, z, pages, L)[None] for c, z in ((kc, ks), (vc, vs)))
         o, _ = ref.attention(q[b, : Hq * D].view(1, 1, Hq, D), k, v, scale, True, L - 1, window, softcap)
         out[b, : Hq * D] = o.reshape(-1).to(out.dtype)
     return out

@@ -17,6 +17,8 @@
 #include <c10/cuda/CUDAGuard.h>
 #include <cuda_fp16.h>
 
+#include <cmath>
+
 #include "common.cuh"
 #include "decode_common.cuh"
 #include "host_utils.h"
@@ -1102,7 +1104,8 @@ at::Tensor kv8_decode_attention(at::Tensor q, at::Tensor kc, at::Tensor ks, at::
                 "kv8_decode_attention: q and out are bf16 [B, >= Hq D], rows on 16-byte boundaries");
   check_ints(slot, kc, B, "kv8_decode_attention: slot [B]");
   check_ints(seqlen, kc, B, "kv8_decode_attention: seqlen [B]");
-  TORCH_CHECK(window >= 0 && window < (int64_t(1) << 31) && softcap >= 0, "kv8_decode_attention: window and softcap");
+  TORCH_CHECK(window >= 0 && window < (int64_t(1) << 31) && softcap >= 0 && std::isfinite(softcap),
+              "kv8_decode_attention: window and softcap");
   const int64_t G = Hq / Hkv, hg = (G + 7) / 8;
   TORCH_CHECK(B <= kMaxSeqs, "kv8_decode_attention: at most 8192 sequences");
   TORCH_CHECK(workspace.device() == kc.device() && workspace.scalar_type() == at::kByte && workspace.is_contiguous() &&
