@@ -10,8 +10,10 @@
 //
 // Positions, slots and lengths are read from device memory, so a captured CUDA
 // graph replays the same launch for any step. A table row, page or position out
-// of range is skipped (appends) or taken as an empty sequence / page 0 (reads)
-// and reported in the device status word, never dereferenced.
+// of range is reported in the device status word and never dereferenced: an
+// append skips the block, a gather reads zeros, attention takes a bad table row
+// for an empty sequence, stops at the table's end and gives the keys of a bad
+// page no weight.
 #include <ATen/ATen.h>
 #include <ATen/cuda/CUDAContext.h>
 #include <c10/cuda/CUDAGuard.h>
@@ -359,8 +361,10 @@ __global__ void __launch_bounds__(kGatherThreads) gather_kernel(GatherParams p) 
 // each in registers keep 64 KB in flight, and the tensor pipe is busy for a sixth
 // of the time); 1 x 100001 keys, 8 KV heads, in 45 us (0.69: a range more or less
 // of 128 keys is 4 % of a CTA's work, and the join adds 3 us); 16 ragged sequences
-// of up to 2304 keys in 14.5 us and 1 x 97 keys in 4.5 us, the chain page -> codes
-// -> products -> sums of eight warps. A ring of asynchronous copies in shared
+// of up to 2304 keys in 14.5 us and 1 x 97 keys (12 heads of 2) in 4.5 us, the chain
+// page -> codes -> products -> sums of eight warps; 6.3 us with a page table of 4096
+// positions, which takes ranges and the join. 64 x 4096 with a softcap 55.2 us, with
+// a window of 2048 31.8 (134 MB, 4.2 TB/s), with D 64 34.4 (135 MB, 3.9 TB/s). A ring of asynchronous copies in shared
 // memory adds instructions and was slower (63 us for 64 x 4096, this form then 55).
 constexpr float kLog2e = 1.4426950408889634f;
 constexpr int kWarps = 8;
@@ -368,7 +372,8 @@ constexpr int kThreads = kWarps * 32;
 constexpr int kMaxCtas = 512;       // parts: two for each CTA
 constexpr int kMaxSeqs = 8192;
 constexpr int kMinSteps = 2;        // of kWarps blocks: shorter ranges cost more to join than they save
-// Page tables of at most so many positions: a CTA for each segment, none cut. 1, 16, 64 and 256 full sequences of 4 KV
+// Page tables (or windows) of at most so many positions: a CTA for each segment, none cut. The host knows the table's
+// width and not the lengths, so short sequences in a wide table, as a server's, go the other way. 1, 16, 64 and 256 full sequences of 4 KV
 // heads, whole / in ranges: 512 keys 6.8 / 8.1, 7.2 / 10.4, 9.6 / 11.5, 36.2 / 37.5 us; 1024 keys 9.4 / 8.8, 9.8 / 11.9,
 // 13.9 / 20.1, 57.0 / 56.1; 2048 keys 14.6 / 9.3, 14.9 / 14.2, 26.4 / 30.9, 100.5 / 94.2.
 constexpr int kWholeKeys = 1024;

@@ -29,11 +29,12 @@ namespace w4 {
 // and is scaled once. The CTAs of a cluster add their sums over distributed
 // shared memory, each its share of the outputs in the order of the columns, so
 // no workspace is needed and the result is the same on every run.
-// Bound by the issue of the unpacking (11 instructions for eight weights, about
-// 125 for a warp's column tile) beside the weights' bytes. Measured, groups of
-// 128: 1 x 3584 -> 37888 (SwiGLU) in 17.9 us, 70.0 MB at 3.92 TB/s (0.60 of a
-// copy's rate; issue slots 60 % busy); 16 rows 24.7 us; 16 x 18944 -> 3584, groups
-// of 64, in 18.8 us; 1 x 1536 -> 2048 in 3.9 us.
+// No unit is at its limit: 16 multiplying warps an SM leave 40 % of the issue slots
+// empty (11 unpacking instructions for eight weights, about 125 for a warp's column
+// tile, wait for one another), and 59 % with 16 rows. Measured, groups of 128:
+// 1 x 3584 -> 37888 (SwiGLU) in 17.9 us, 70.0 MB at 3.92 TB/s (0.60 of a copy's
+// rate); 16 rows 24.7 us; 16 x 18944 -> 3584, groups of 64, in 18.8 us;
+// 1 x 1536 -> 2048 in 3.9 us.
 constexpr int kWarps = 8;                   // that multiply
 constexpr int kThreads = kWarps * 32 + 32;
 constexpr int kPair = 2;                    // column tiles of a ring stage
@@ -278,7 +279,9 @@ static void launch_group(LinearParams& p, cudaStream_t st) {
 }
 
 // out [N, K] bf16 = code * scale, for products of more rows than a decode
-// batch: one thread a word of eight elements.
+// batch: one thread a word of eight elements. Bound by bytes written in pieces of
+// eight, two of a row to a thread. Measured, groups of 128: 37888 x 3584 in 87 us
+// (339 MB at 3.9 TB/s, 0.59 of a copy's rate).
 __global__ void __launch_bounds__(256) dequant_kernel(Weight w, int64_t words, __nv_bfloat16* __restrict__ out) {
   const int64_t i = (int64_t)blockIdx.x * blockDim.x + threadIdx.x;
   if (i >= words) return;
